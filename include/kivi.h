@@ -343,6 +343,108 @@ kivi_status kivi_runtime_decode_device(kivi_runtime* rt, const float* key, size_
                                        float* out, size_t out_len, void* stream,
                                        kivi_error* err);
 
+/* ---------------------------------------------------------------- paged cache
+ * Extension, no reference counterpart: a pool of pages that holds the quantized tokens of many
+ * sequences of any lengths, for servers that batch continuously. A sequence of n tokens is, bit for
+ * bit, what a KiviCache of one batch element holds after n appended tokens: its first n / R * R keys
+ * and its first n - R values are quantized (R = residual_length), the rest are rows in the caller's
+ * type. All of that follows from n, so the cache keeps no lengths: the caller passes them with every
+ * call, in device memory, along with which pages and which window each sequence has.
+ *
+ * Only device pointers, and nothing but enqueued work: no call on a live cache allocates, waits or
+ * keeps anything, so all may be captured into a graph (whose replays read the arrays' contents of
+ * that moment) and made on any stream. The caller orders calls that write a sequence with other calls
+ * on that sequence; calls on other sequences may overlap. */
+typedef struct kivi_paged kivi_paged;
+
+/* Element type of the rows: keys, values, queries, outputs and the windows. Quantization and softmax
+ * run in f32 whatever the type; an output is rounded once. */
+typedef enum kivi_dtype { KIVI_DTYPE_F32 = 0, KIVI_DTYPE_F16 = 1, KIVI_DTYPE_BF16 = 2 } kivi_dtype;
+
+/* num_pages pages of page_tokens tokens (all KV heads; a multiple of 32 and of group_size, else
+ * TokenGroup{page_tokens, lcm(32, group_size)}) and num_slots windows. head_dim is at most 256 and
+ * lcm(32, group_size) at most 512 (Unsupported beyond). */
+kivi_status kivi_paged_new(const kivi_config* config, size_t num_kv_heads, size_t head_dim,
+                           int32_t dtype, size_t page_tokens, size_t num_pages, size_t num_slots,
+                           kivi_paged** out, kivi_error* err);
+/* Waits for the device's work first. */
+void kivi_paged_free(kivi_paged* cache);
+kivi_config kivi_paged_config(const kivi_paged* cache);
+size_t kivi_paged_num_kv_heads(const kivi_paged* cache);
+size_t kivi_paged_head_dim(const kivi_paged* cache);
+int32_t kivi_paged_dtype(const kivi_paged* cache);
+size_t kivi_paged_page_tokens(const kivi_paged* cache);
+size_t kivi_paged_num_pages(const kivi_paged* cache);
+size_t kivi_paged_num_slots(const kivi_paged* cache);
+/* Device memory of the pages and the windows. */
+size_t kivi_paged_device_bytes(const kivi_paged* cache);
+
+/* A ragged batch. The four arrays are device memory, read when the work runs:
+ *   slots   [sequences]      window of each sequence, in [0, num_slots); in one call that appends,
+ *                            no two sequences have the same one
+ *   lengths [sequences]      tokens of the sequence that the cache holds
+ *   starts  [sequences + 1]  rows of sequence i in the call's tensors: [starts[i], starts[i + 1])
+ *   pages   [sequences][pages_per_sequence]  page of tokens p * page_tokens ..; two sequences may
+ *                            share pages that neither writes
+ * `rows` is the number of rows of the call's tensors; rows behind the last sequence are left as they
+ * were. `max_rows` bounds the rows of one sequence (0: `rows`); a sequence with more is cut to its
+ * first max_rows. `max_length` is the longest length to plan for (0: the table's); longer ones are
+ * right all the same. Values outside their ranges do no harm: a sequence whose slot is none of the
+ * cache's counts as holding nothing and is not appended to; the tokens of a page that is none of
+ * the pool's (-1, say) are not written, read as zeros and are seen by no query; a length below 0
+ * is 0; starts are cut to [0, rows]. At most 65535 sequences and 2^24 rows of one sequence. */
+typedef struct kivi_paged_batch {
+  size_t sequences;
+  const int32_t* slots;
+  const int32_t* lengths;
+  const int32_t* starts;
+  const int32_t* pages;
+  size_t pages_per_sequence;
+  size_t rows;
+  size_t max_rows;
+  size_t max_length;
+} kivi_paged_batch;
+
+/* Tensors of rows are [rows][heads][head_dim] of the cache's dtype: pointer, element count, and
+ * elements from row to row (`*_stride`, 0: heads * head_dim). Heads lie next to each other. A stride
+ * under heads * head_dim, or a count under (rows - 1) * stride + heads * head_dim, is a Shape error.
+ * Any alignment of the element type works; rows on 16 bytes are read and written faster.
+ *
+ * Appends the batch's new rows behind lengths[i] tokens. Up to residual_length rows a sequence may be
+ * appended again, or others in their place, by passing the old length: the windows keep every row
+ * that such a call quantizes (drafted tokens are taken back so). */
+kivi_status kivi_paged_append_device(kivi_paged* cache, const kivi_paged_batch* batch,
+                                     const void* keys, size_t keys_len, size_t keys_stride,
+                                     const void* values, size_t values_len, size_t values_stride,
+                                     void* stream, kivi_error* err);
+/* Reads tokens first[i] + r of each sequence (first: device [sequences], null: 0) into its row r. Tokens at
+ * or behind lengths[i] read as zeros. */
+kivi_status kivi_paged_read_device(const kivi_paged* cache, const kivi_paged_batch* batch,
+                                   const int32_t* first, void* keys, size_t keys_len,
+                                   size_t keys_stride, void* values, size_t values_len,
+                                   size_t values_stride, void* stream, kivi_error* err);
+
+/* Bytes of workspace that kivi_paged_attention_device wants for a batch of these sizes (its arrays
+ * are not read). */
+kivi_status kivi_paged_attention_workspace(const kivi_paged* cache, const kivi_paged_batch* batch,
+                                           size_t num_q_heads, size_t* bytes, kivi_error* err);
+/* Causal attention of each sequence's m new tokens (queries and out: [rows][num_q_heads][head_dim])
+ * over its L tokens; query row j stands at position L - m + j. With keys and values null the new
+ * tokens are in the cache already (lengths[i] = L counts them); otherwise they are these rows,
+ * exactly as given, behind the lengths[i] = L - m cached tokens, and are appended by a call of their own.
+ * With window != 0 a query at position p sees the tokens t <= p with t > p - window or t < sinks;
+ * pages that hold no such token are not read. A row that sees nothing is zero. The workspace is the
+ * caller's (16-byte aligned; too small is Capacity{needed, given}); calls that may overlap need one
+ * each. */
+kivi_status kivi_paged_attention_device(const kivi_paged* cache, const kivi_paged_batch* batch,
+                                        const void* queries, size_t queries_len,
+                                        size_t queries_stride, size_t num_q_heads, const void* keys,
+                                        size_t keys_len, size_t keys_stride, const void* values,
+                                        size_t values_len, size_t values_stride, float scale,
+                                        size_t window, size_t sinks, void* out, size_t out_len,
+                                        size_t out_stride, void* workspace, size_t workspace_bytes,
+                                        void* stream, kivi_error* err);
+
 /* ---------------------------------------------------------------- QualityGuard */
 /* QualityGuard (src/guard.rs:37-258): a cache plus the fp32 tape of every appended token;
    after each key flush the guard scores cache attention against fp32 attention over the tape

@@ -23,6 +23,7 @@
 
 #include "kivi.h"
 #include "common.hpp"
+#include "paged.hpp"
 
 namespace kivi {
 namespace {
@@ -1549,6 +1550,21 @@ Status quantized_read(const kivi_quantized* q, void* out, size_t out_len, size_t
 // QualityGuard (src/guard.rs:37-258): the resident cache plus the fp32 tape of every appended
 // token, here on the device ([units][cap][D], grown by doubling) so the fp32 attention it is
 // scored against runs on the attention kernels (tape rows as the suffix of an empty cache).
+struct kivi_paged {
+  kivi_config cfg{};
+  int device = 0;
+  PagedGeometry geo{};
+  DevBuf pages, kwin, vwin;
+  PagedView view() const {
+    PagedView v;
+    v.geo = geo;
+    v.pages = pages.as<uint32_t>();
+    v.kwin = kwin.p;
+    v.vwin = vwin.p;
+    return v;
+  }
+};
+
 struct kivi_guard {
   kivi_cache* cache = nullptr;
   DevBuf tk, tv;
@@ -1563,6 +1579,123 @@ struct kivi_guard {
 };
 
 namespace {
+
+// ---------------------------------------------------------------- paged cache
+
+// Threads of a launch's first grid dimension stay under 2^32 up to this many rows of one sequence.
+constexpr size_t kMaxPagedRows = (size_t)1 << 24;
+constexpr size_t kMaxGridYZ = 65535;  // sequences and heads are grid dimensions
+
+Status create_paged(const kivi_config* config, size_t heads, size_t head_dim, int32_t dtype, size_t page_tokens,
+                    size_t num_pages, size_t num_slots, kivi_paged** out, kivi_paged* c) {
+  KIVI_TRY(need(config, "config"));
+  KIVI_TRY(check_config(*config));
+  if (heads == 0) return Err(KIVI_ERR_ZERO_DIMENSION, 0, 0, "num_kv_heads");
+  if (head_dim == 0 || head_dim % config->group_size != 0)
+    return Err(KIVI_ERR_HEAD_DIM, head_dim, config->group_size);
+  if (dtype != KIVI_DTYPE_F32 && dtype != KIVI_DTYPE_F16 && dtype != KIVI_DTYPE_BF16)
+    return Err(KIVI_ERR_UNSUPPORTED, static_cast<uint64_t>(static_cast<int64_t>(dtype)), KIVI_DTYPE_BF16, "dtype");
+  if (head_dim > kPagedMaxHeadDim) return Err(KIVI_ERR_UNSUPPORTED, head_dim, kPagedMaxHeadDim, "head_dim");
+  if (heads > kMaxGridYZ) return Err(KIVI_ERR_UNSUPPORTED, heads, kMaxGridYZ, "num_kv_heads");
+  if (config->residual_length > kMaxResidual)
+    return Err(KIVI_ERR_UNSUPPORTED, config->residual_length, kMaxResidual, "residual_length");
+  const uint64_t span = lcm64(kPagedBlock, config->group_size);
+  if (span > kPagedMaxSpan) return Err(KIVI_ERR_UNSUPPORTED, span, kPagedMaxSpan, "lcm(32, group_size)");
+  if (page_tokens == 0 || page_tokens % span != 0) return Err(KIVI_ERR_TOKEN_GROUP, page_tokens, span);
+  if (page_tokens > kMaxResidual) return Err(KIVI_ERR_UNSUPPORTED, page_tokens, kMaxResidual, "page_tokens");
+  if (num_pages == 0) return Err(KIVI_ERR_ZERO_DIMENSION, 0, 0, "num_pages");
+  if (num_slots == 0) return Err(KIVI_ERR_ZERO_DIMENSION, 0, 0, "num_slots");
+  if (num_pages > INT32_MAX) return Err(KIVI_ERR_UNSUPPORTED, num_pages, INT32_MAX, "num_pages");
+  if (num_slots > INT32_MAX) return Err(KIVI_ERR_UNSUPPORTED, num_slots, INT32_MAX, "num_slots");
+  KIVI_TRY(need(out, "out"));
+  PagedGeometry& g = c->geo;
+  g.bits = config->bits;
+  g.G = static_cast<uint32_t>(config->group_size);
+  g.R = static_cast<uint32_t>(config->residual_length);
+  g.D = static_cast<uint32_t>(head_dim);
+  g.DP = (g.D + 31) / 32 * 32;
+  g.heads = static_cast<uint32_t>(heads);
+  g.P = static_cast<uint32_t>(page_tokens);
+  g.span = static_cast<uint32_t>(span);
+  g.pages = static_cast<uint32_t>(num_pages);
+  g.slots = static_cast<uint32_t>(num_slots);
+  g.type = static_cast<uint32_t>(dtype);
+  // words of a record: at most 256 tokens' worth of f32 pairs per token and channel
+  size_t record, pages_bytes, rows, window_bytes;
+  KIVI_TRY(mul4(page_tokens, g.DP, 32, 1, &record));
+  if (record > UINT32_MAX) return Err(KIVI_ERR_UNSUPPORTED, page_tokens, UINT32_MAX / (32 * g.DP), "page_tokens");
+  KIVI_TRY(mul4(num_pages, heads, g.record_words(), 4, &pages_bytes));
+  KIVI_TRY(mul4(num_slots, heads, 2 * config->residual_length, 1, &rows));
+  KIVI_TRY(mul4(rows, head_dim, g.type_bytes(), 1, &window_bytes));
+  c->cfg = *config;
+  KIVI_TRY(current_device(&c->device));
+  KIVI_TRY(c->pages.alloc(pages_bytes, nullptr, "paged cache"));
+  KIVI_TRY(c->kwin.alloc(window_bytes, nullptr, "paged cache windows"));
+  KIVI_TRY(c->vwin.alloc(window_bytes, nullptr, "paged cache windows"));
+  // the channels behind head_dim are never written and have to be zero
+  HIP_TRY(launch_fill_zero(c->pages.as<float>(), pages_bytes / 4, nullptr), "paged cache");
+  return sync(nullptr, "paged cache");
+}
+
+Status paged_batch(const kivi_paged& c, const kivi_paged_batch* in, PagedBatch* b) {
+  KIVI_TRY(need(in, "batch"));
+  if (in->sequences > kMaxGridYZ) return Err(KIVI_ERR_UNSUPPORTED, in->sequences, kMaxGridYZ, "sequences");
+  if (in->rows > INT32_MAX) return Err(KIVI_ERR_UNSUPPORTED, in->rows, INT32_MAX, "rows");
+  const size_t most = in->max_rows == 0 ? in->rows : std::min(in->max_rows, in->rows);
+  if (most > kMaxPagedRows) return Err(KIVI_ERR_UNSUPPORTED, most, kMaxPagedRows, "max_rows");
+  if (in->pages_per_sequence > INT32_MAX)
+    return Err(KIVI_ERR_UNSUPPORTED, in->pages_per_sequence, INT32_MAX, "pages_per_sequence");
+  if (in->sequences != 0) {
+    KIVI_TRY(need(in->slots, "slots"));
+    KIVI_TRY(need(in->lengths, "lengths"));
+    KIVI_TRY(need(in->starts, "starts"));
+    if (in->pages_per_sequence != 0) KIVI_TRY(need(in->pages, "pages"));
+  }
+  const uint64_t held = (uint64_t)in->pages_per_sequence * c.geo.P + c.geo.R;
+  b->slots = in->slots;
+  b->lengths = in->lengths;
+  b->starts = in->starts;
+  b->table = in->pages;
+  b->sequences = static_cast<uint32_t>(in->sequences);
+  b->per_sequence = static_cast<uint32_t>(in->pages_per_sequence);
+  b->rows = static_cast<int64_t>(in->rows);
+  b->max_rows = static_cast<uint32_t>(most);
+  b->max_length = in->max_length == 0 ? held : std::min<uint64_t>(in->max_length, held);
+  return Status{};
+}
+
+Status paged_rows(const kivi_paged& c, const PagedBatch& b, size_t heads, const void* p, size_t len, size_t stride,
+                  const char* name, PagedRows* out) {
+  const size_t size = c.geo.type_bytes();
+  size_t row, expected = 0;
+  KIVI_TRY(mul(heads, c.geo.D, &row));
+  if (stride == 0) stride = row;
+  if (stride < row) return Err(KIVI_ERR_SHAPE, row, stride);
+  if (b.rows != 0) {
+    KIVI_TRY(need(p, name));
+    KIVI_TRY(mul(static_cast<size_t>(b.rows) - 1, stride, &expected));
+    if (expected > SIZE_MAX / 8 - row) return Err(KIVI_ERR_CAPACITY, expected, SIZE_MAX / 8 - row);
+    expected += row;
+  }
+  if (len < expected) return Err(KIVI_ERR_SHAPE, expected, len);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+  if (at % size != 0) return Err(KIVI_ERR_UNSUPPORTED, at % size, 0, "address % element size");
+  out->p = p;
+  out->stride = stride;
+  out->vec = at % 16 == 0 && stride * size % 16 == 0 && c.geo.D * size % 16 == 0;
+  return Status{};
+}
+
+// Rows of one KV head are counted in 32 bits.
+Status paged_query_heads(const kivi_paged& c, const PagedBatch& b, size_t qh) {
+  if (qh == 0 || qh % c.geo.heads != 0) return Err(KIVI_ERR_QUERY_HEADS, qh, c.geo.heads);
+  const size_t gq = qh / c.geo.heads;
+  if (gq > kMaxGridYZ) return Err(KIVI_ERR_UNSUPPORTED, gq, kMaxGridYZ, "num_q_heads/num_kv_heads");
+  if (gq * b.max_rows > (size_t)1 << 30)
+    return Err(KIVI_ERR_UNSUPPORTED, gq * b.max_rows, (size_t)1 << 30, "max_rows*(num_q_heads/num_kv_heads)");
+  return Status{};
+}
+
 
 // next_bits / next_residual (src/guard.rs:261-289).
 bool guard_next_bits(uint8_t current, uint8_t max_bits, uint8_t* next) {
@@ -2109,6 +2242,129 @@ kivi_status kivi_runtime_decode_device(kivi_runtime* rt, const float* key, size_
   if (st != KIVI_OK) return st;
   return kivi_cache_attention_device(&rt->cache, query, query_len, num_q_heads, scale, out,
                                      out_len, stream, err);
+}
+
+kivi_status kivi_paged_new(const kivi_config* config, size_t num_kv_heads, size_t head_dim,
+                           int32_t dtype, size_t page_tokens, size_t num_pages, size_t num_slots,
+                           kivi_paged** out, kivi_error* err) {
+  return guarded(err, [&] {
+    auto c = std::make_unique<kivi_paged>();
+    KIVI_TRY(create_paged(config, num_kv_heads, head_dim, dtype, page_tokens, num_pages, num_slots, out, c.get()));
+    *out = c.release();
+    return Status{};
+  });
+}
+
+void kivi_paged_free(kivi_paged* cache) {
+  if (cache == nullptr) return;
+  DeviceScope scope(cache->device);
+  QuietDevice quiet;
+  delete cache;
+}
+
+kivi_config kivi_paged_config(const kivi_paged* c) { return c->cfg; }
+size_t kivi_paged_num_kv_heads(const kivi_paged* c) { return c->geo.heads; }
+size_t kivi_paged_head_dim(const kivi_paged* c) { return c->geo.D; }
+int32_t kivi_paged_dtype(const kivi_paged* c) { return static_cast<int32_t>(c->geo.type); }
+size_t kivi_paged_page_tokens(const kivi_paged* c) { return c->geo.P; }
+size_t kivi_paged_num_pages(const kivi_paged* c) { return c->geo.pages; }
+size_t kivi_paged_num_slots(const kivi_paged* c) { return c->geo.slots; }
+size_t kivi_paged_device_bytes(const kivi_paged* c) {
+  return c ? c->pages.bytes + c->kwin.bytes + c->vwin.bytes : 0;
+}
+
+kivi_status kivi_paged_append_device(kivi_paged* cache, const kivi_paged_batch* batch,
+                                     const void* keys, size_t keys_len, size_t keys_stride,
+                                     const void* values, size_t values_len, size_t values_stride,
+                                     void* stream, kivi_error* err) {
+  return guarded(err, [&] {
+    KIVI_TRY(need(cache, "cache"));
+    PagedBatch b;
+    PagedRows k, v;
+    KIVI_TRY(paged_batch(*cache, batch, &b));
+    KIVI_TRY(paged_rows(*cache, b, cache->geo.heads, keys, keys_len, keys_stride, "keys", &k));
+    KIVI_TRY(paged_rows(*cache, b, cache->geo.heads, values, values_len, values_stride, "values", &v));
+    if (b.max_rows == 0 || b.sequences == 0) return Status{};
+    DeviceScope scope(cache->device);
+    HIP_TRY(launch_paged_append(cache->view(), b, k, v, static_cast<hipStream_t>(stream)), "paged append");
+    return Status{};
+  });
+}
+
+kivi_status kivi_paged_read_device(const kivi_paged* cache, const kivi_paged_batch* batch,
+                                   const int32_t* first, void* keys, size_t keys_len,
+                                   size_t keys_stride, void* values, size_t values_len,
+                                   size_t values_stride, void* stream, kivi_error* err) {
+  return guarded(err, [&] {
+    KIVI_TRY(need(cache, "cache"));
+    PagedBatch b;
+    PagedRows k, v;
+    KIVI_TRY(paged_batch(*cache, batch, &b));
+    KIVI_TRY(paged_rows(*cache, b, cache->geo.heads, keys, keys_len, keys_stride, "keys", &k));
+    KIVI_TRY(paged_rows(*cache, b, cache->geo.heads, values, values_len, values_stride, "values", &v));
+    if (b.max_rows == 0 || b.sequences == 0) return Status{};
+    DeviceScope scope(cache->device);
+    HIP_TRY(launch_paged_read(cache->view(), b, first, k, v, static_cast<hipStream_t>(stream)), "paged read");
+    return Status{};
+  });
+}
+
+kivi_status kivi_paged_attention_workspace(const kivi_paged* cache, const kivi_paged_batch* batch,
+                                           size_t num_q_heads, size_t* bytes, kivi_error* err) {
+  return guarded(err, [&] {
+    KIVI_TRY(need(cache, "cache"));
+    KIVI_TRY(need(bytes, "bytes"));
+    PagedBatch b;
+    KIVI_TRY(paged_batch(*cache, batch, &b));
+    KIVI_TRY(paged_query_heads(*cache, b, num_q_heads));
+    *bytes = b.max_rows == 0 || b.sequences == 0
+                 ? 0
+                 : paged_attention_workspace(cache->geo, b, static_cast<uint32_t>(num_q_heads));
+    return Status{};
+  });
+}
+
+kivi_status kivi_paged_attention_device(const kivi_paged* cache, const kivi_paged_batch* batch,
+                                        const void* queries, size_t queries_len,
+                                        size_t queries_stride, size_t num_q_heads, const void* keys,
+                                        size_t keys_len, size_t keys_stride, const void* values,
+                                        size_t values_len, size_t values_stride, float scale,
+                                        size_t window, size_t sinks, void* out, size_t out_len,
+                                        size_t out_stride, void* workspace, size_t workspace_bytes,
+                                        void* stream, kivi_error* err) {
+  return guarded(err, [&] {
+    KIVI_TRY(need(cache, "cache"));
+    PagedAttention a{};
+    KIVI_TRY(paged_batch(*cache, batch, &a.b));
+    KIVI_TRY(paged_query_heads(*cache, a.b, num_q_heads));
+    KIVI_TRY(paged_rows(*cache, a.b, num_q_heads, queries, queries_len, queries_stride, "queries", &a.query));
+    if (keys != nullptr || values != nullptr) {
+      KIVI_TRY(paged_rows(*cache, a.b, cache->geo.heads, keys, keys_len, keys_stride, "keys", &a.keys));
+      KIVI_TRY(paged_rows(*cache, a.b, cache->geo.heads, values, values_len, values_stride, "values", &a.values));
+    }
+    PagedRows to;
+    KIVI_TRY(paged_rows(*cache, a.b, num_q_heads, out, out_len, out_stride, "out", &to));
+    if (a.b.max_rows == 0 || a.b.sequences == 0) return Status{};
+    a.c = cache->view();
+    a.out = out;
+    a.out_stride = to.stride;
+    a.out_vec = to.vec;
+    a.qh = static_cast<uint32_t>(num_q_heads);
+    a.scale = scale;
+    // beyond any position
+    a.window = std::min<size_t>(window, (size_t)1 << 40);
+    a.sinks = std::min<size_t>(sinks, (size_t)1 << 40);
+    const size_t bytes = paged_attention_workspace(cache->geo, a.b, a.qh);
+    if (workspace_bytes < bytes) return Err(KIVI_ERR_CAPACITY, bytes, workspace_bytes, "workspace");
+    if (bytes != 0) {
+      KIVI_TRY(need(workspace, "workspace"));
+      if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
+        return Err(KIVI_ERR_UNSUPPORTED, reinterpret_cast<uintptr_t>(workspace) % 16, 0, "workspace % 16");
+    }
+    DeviceScope scope(cache->device);
+    HIP_TRY(launch_paged_attention(a, static_cast<float*>(workspace), static_cast<hipStream_t>(stream)), "paged attention");
+    return Status{};
+  });
 }
 
 kivi_status kivi_guard_new(const kivi_config* config, size_t batch, size_t num_kv_heads,

@@ -20,10 +20,6 @@ namespace {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ float scale_of(float span, float levels) {
-  return span == 0.0f ? 0.0f : span / levels;
-}
-
 __device__ __forceinline__ uint32_t quant_code(float x, float zero, float scale, float levels) {
   if (scale == 0.0f) return 0u;
   float r = rintf((x - zero) / scale);
@@ -33,28 +29,6 @@ __device__ __forceinline__ uint32_t quant_code(float x, float zero, float scale,
     r = levels;
   }
   return static_cast<uint32_t>(r);
-}
-
-// Reciprocal for quant_code_fast: 0 for a zero scale (every code is then 0).
-__device__ __forceinline__ float quant_inv(float scale) {
-  return scale == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(scale);
-}
-
-// quant_code from a reciprocal, bit-identical to it. With v_rcp_f32's 1-ulp reciprocal,
-// q = (x - zero) * inv lies within q * 2^-22 <= 2^-14 of the correctly rounded quotient
-// (x - zero) / scale (0 <= x - zero <= span keeps q <= levels (1 + 2^-22) <= 256), so both
-// round to the same integer unless q is within 2^-12 of a half-integer: |q - rint(q)| >=
-// 0.5 - 2^-12, which is also true of a non-finite q (inv = inf); those lanes divide.
-// x >= zero here (zero is the group minimum), so r >= 0 and the clamp is an integer min.
-__device__ __forceinline__ uint32_t quant_code_fast(float x, float zero, float scale, float inv,
-                                                    uint32_t levels) {
-#pragma clang fp contract(off)
-  const float d = x - zero;
-  const float q = d * inv;
-  float r = rintf(q);
-  if (!(fabsf(q - r) < 0.5f - 0x1p-12f)) r = scale == 0.0f ? 0.0f : rintf(d / scale);
-  const uint32_t u = static_cast<uint32_t>(r);
-  return u < levels ? u : levels;
 }
 
 // DPP lane exchanges inside rows of 16 lanes (every lane active): quad_perm xor 1 and xor 2,

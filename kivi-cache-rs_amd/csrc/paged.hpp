@@ -1,0 +1,163 @@
+// paged.hpp — device layout of the paged KIVI cache and the launch interface shared by its
+// kernels (kernels_paged.hip, kernels_paged_attn.hip) and the host (host.cpp).
+//
+// A pool of pages holds the quantized tokens of many sequences; a table gives each sequence's
+// pages. How much of a sequence is quantized follows from its length n alone, as in a KiviCache
+// that got its tokens in any pieces: the first n / R * R keys and the first n - R values. The last
+// tokens also lie in windows of the caller's type, 2 R rows per slot and KV head for keys and for
+// values (token t in row t % (2 R)). R rows would do for the present; 2 R leave every row that an
+// append of up to R tokens quantizes where it was, so that such an append may be repeated or taken
+// back by passing the old length (drafted tokens that were refused), and so that it has no reads
+// that its own writes could overtake.
+//
+// Page p, KV head h: one record at pages + (p * heads + h) * record, four arrays in this order:
+//
+//   key codes    u32 [P/32] blocks   key block: lane-major fragments, see below
+//   key params   f32 [P/G][DP][2]    (scale, zero) per (group, channel)
+//   value codes  u32 [P/32] blocks
+//   value params f32 [P][D/G][2]     (scale, zero) per (token, channel group)
+//
+// DP is D rounded up to 32 (codes and key params of the channels behind D stay zero). A block of 32
+// tokens is stored as the 64 lanes of a wave read it for the matrix cores: lane L holds 2S
+// fragments of eight codes (S = DP/32), its words contiguous. With q = L / 16, l = L % 16:
+//
+//   keys    fragment f = 16-token half * S + s: token half*16 + l, channels 8S q + 8 s + (0..7)
+//   values  fragment f: channel 16 f + l, tokens 4q + (0..3) and 16 + 4q + (0..3)
+//
+// The value tokens follow the accumulator layout of the 16-row matrix instructions (row 4q + i of
+// each 16-token tile), so softmax weights go from one product to the next in the lane that has
+// them. Inside the words, element j of fragment f lies where the packed fp4 / fp8 converters take
+// it without shuffling: 2 bits: word f/2, bit 4j + 2(f%2); 4 bits: word f, bit 8(j%4) + 4(j/4);
+// 8 bits: word 2f + j/4, bit 8(j%4).
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+namespace kivi {
+
+constexpr uint32_t kPagedBlock = 32;       // tokens per code block
+constexpr uint32_t kPagedMaxHeadDim = 256;
+constexpr uint32_t kPagedMaxSpan = 512;    // lcm(32, G): tokens a key-quantizing workgroup stages in LDS
+
+enum PagedType : uint32_t { kPagedF32 = 0, kPagedF16 = 1, kPagedBF16 = 2 };
+
+struct PagedGeometry {
+  uint32_t bits, G, R, D, DP;
+  uint32_t heads;
+  uint32_t P;      // tokens per page
+  uint32_t span;   // lcm(32, G)
+  uint32_t pages;  // pages of the pool
+  uint32_t slots;  // windows
+  uint32_t type;   // PagedType
+
+  __host__ __device__ uint32_t S() const { return DP / 32; }
+  __host__ __device__ uint32_t ncg() const { return D / G; }
+  __host__ __device__ uint32_t levels() const { return (1u << bits) - 1u; }
+  __host__ __device__ uint32_t lane_words() const { return DP / 32 * bits / 2; }
+  __host__ __device__ uint32_t block_words() const { return DP * bits; }  // 32 tokens * DP * bits / 32
+  __host__ __device__ uint32_t kparams_at() const { return P / 32 * block_words(); }  // in words, from the record
+  __host__ __device__ uint32_t vcodes_at() const { return kparams_at() + P / G * DP * 2; }
+  __host__ __device__ uint32_t vparams_at() const { return vcodes_at() + P / 32 * block_words(); }
+  __host__ __device__ uint32_t record_words() const { return vparams_at() + P * ncg() * 2; }
+  __host__ __device__ uint64_t page_words() const { return (uint64_t)heads * record_words(); }
+  __host__ __device__ uint64_t window_rows() const { return (uint64_t)slots * heads * 2 * R; }
+  __host__ __device__ uint32_t type_bytes() const { return type == kPagedF32 ? 4u : 2u; }
+};
+
+struct PagedView {
+  PagedGeometry geo;
+  uint32_t* pages;
+  void* kwin;  // [slots][heads][2R][D]
+  void* vwin;
+};
+
+// A ragged batch: device arrays of a kivi_paged_batch and its bounds.
+struct PagedBatch {
+  const int32_t* slots;
+  const int32_t* lengths;
+  const int32_t* starts;
+  const int32_t* table;
+  uint32_t sequences;
+  uint32_t per_sequence;  // table entries of a sequence
+  int64_t rows;
+  uint32_t max_rows;      // longest chunk (the host's bound; longer ones are cut to it)
+  uint64_t max_length;    // longest cached length expected (for the grids only)
+};
+
+// One sequence of a batch as the kernels see it: whatever the device arrays hold, the ranges stay
+// inside the tensors, and a page or slot outside the pool is no page or slot.
+struct PagedSequence {
+  int64_t n;       // cached tokens
+  int64_t row0;    // first row of the new tokens
+  uint32_t m;      // new tokens
+  int32_t slot;    // -1: none
+  const int32_t* table;
+};
+
+__device__ __forceinline__ PagedSequence paged_sequence(const PagedBatch& b, const PagedGeometry& g, uint32_t i) {
+  PagedSequence s;
+  const int32_t n = b.lengths[i], slot = b.slots[i];
+  const int64_t a0 = b.starts[i], a1 = b.starts[i + 1];
+  s.slot = slot >= 0 && (uint32_t)slot < g.slots ? slot : -1;
+  s.n = n > 0 && s.slot >= 0 ? n : 0;
+  s.row0 = a0 < 0 ? 0 : a0 < b.rows ? a0 : b.rows;
+  const int64_t end = a1 < s.row0 ? s.row0 : a1 < b.rows ? a1 : b.rows;
+  const int64_t m = end - s.row0;
+  s.m = m < (int64_t)b.max_rows ? (uint32_t)m : b.max_rows;
+  s.table = b.table + (uint64_t)i * b.per_sequence;
+  return s;
+}
+
+// Record of (page of token t, head), or null where the sequence has no such page.
+__device__ __forceinline__ uint32_t* paged_record(const PagedView& c, const PagedBatch& b, const PagedSequence& s,
+                                                  uint32_t head, int64_t t) {
+  const uint64_t p = (uint64_t)t / c.geo.P;
+  if (p >= b.per_sequence) return nullptr;
+  const int32_t page = s.table[p];
+  if (page < 0 || (uint32_t)page >= c.geo.pages) return nullptr;
+  return c.pages + ((uint64_t)(uint32_t)page * c.geo.heads + head) * c.geo.record_words();
+}
+
+__host__ __device__ inline int64_t paged_kq(const PagedGeometry& g, int64_t n) { return n / g.R * g.R; }
+__host__ __device__ inline int64_t paged_vq(const PagedGeometry& g, int64_t n) { return n > g.R ? n - g.R : 0; }
+
+// Word (of a lane's words) and bit of element j of fragment f.
+__host__ __device__ inline uint32_t paged_word(uint32_t bits, uint32_t f, uint32_t j) {
+  return bits == 2 ? f >> 1 : bits == 4 ? f : 2 * f + (j >> 2);
+}
+__host__ __device__ inline uint32_t paged_bit(uint32_t bits, uint32_t f, uint32_t j) {
+  return bits == 2 ? 4 * j + 2 * (f & 1) : bits == 4 ? 8 * (j & 3) + 4 * (j >> 2) : 8 * (j & 3);
+}
+
+// Rows of a ragged tensor: row r, head h at p + r * stride + h * D (in elements). `vec`: every row
+// of a head starts on 16 bytes (32 for f32 would not be needed: it is read in halves).
+struct PagedRows {
+  const void* p;
+  uint64_t stride;
+  uint32_t vec;
+};
+
+hipError_t launch_paged_append(const PagedView& c, const PagedBatch& b, PagedRows keys, PagedRows values,
+                               hipStream_t stream);
+// Rows starts[i] + r of sequence i <- token first[i] + r (first null: 0).
+hipError_t launch_paged_read(const PagedView& c, const PagedBatch& b, const int32_t* first, PagedRows keys,
+                             PagedRows values, hipStream_t stream);
+
+struct PagedAttention {
+  PagedView c;
+  PagedBatch b;
+  PagedRows query, keys, values;  // keys.p null: the new tokens are cached already
+  void* out;
+  uint64_t out_stride;
+  uint32_t out_vec;
+  uint32_t qh;
+  float scale;
+  uint64_t window, sinks;  // window 0: none
+};
+size_t paged_attention_workspace(const PagedGeometry& g, const PagedBatch& b, uint32_t qh);
+hipError_t launch_paged_attention(const PagedAttention& a, float* workspace, hipStream_t stream);
+
+}  // namespace kivi

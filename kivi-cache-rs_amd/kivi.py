@@ -97,6 +97,20 @@ class _FlushCheck(C.Structure):
     ]
 
 
+class _PagedBatch(C.Structure):
+    _fields_ = [
+        ("sequences", C.c_size_t),
+        ("slots", C.c_void_p),
+        ("lengths", C.c_void_p),
+        ("starts", C.c_void_p),
+        ("pages", C.c_void_p),
+        ("pages_per_sequence", C.c_size_t),
+        ("rows", C.c_size_t),
+        ("max_rows", C.c_size_t),
+        ("max_length", C.c_size_t),
+    ]
+
+
 # Variant names of KiviError (reference src/error.rs:5-45) by status code.
 VARIANTS = {
     1: "InvalidBits",
@@ -287,6 +301,36 @@ _DEVICE_SIGS = {
     "cache_export_streams_device": (
         C.c_int,
         [_P, _P, _SZ, _P, _SZ, _P, _SZ, _P, _SZ, _P, _ERRP],
+    ),
+    "paged_new": (
+        C.c_int,
+        [C.POINTER(_Config), _SZ, _SZ, C.c_int32, _SZ, _SZ, _SZ, C.POINTER(_P), _ERRP],
+    ),
+    "paged_free": (None, [_P]),
+    "paged_config": (_Config, [_P]),
+    "paged_num_kv_heads": (_SZ, [_P]),
+    "paged_head_dim": (_SZ, [_P]),
+    "paged_dtype": (C.c_int32, [_P]),
+    "paged_page_tokens": (_SZ, [_P]),
+    "paged_num_pages": (_SZ, [_P]),
+    "paged_num_slots": (_SZ, [_P]),
+    "paged_device_bytes": (_SZ, [_P]),
+    "paged_append_device": (
+        C.c_int,
+        [_P, C.POINTER(_PagedBatch), _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _ERRP],
+    ),
+    "paged_read_device": (
+        C.c_int,
+        [_P, C.POINTER(_PagedBatch), _P, _P, _SZ, _SZ, _P, _SZ, _SZ, _P, _ERRP],
+    ),
+    "paged_attention_workspace": (
+        C.c_int,
+        [_P, C.POINTER(_PagedBatch), _SZ, C.POINTER(_SZ), _ERRP],
+    ),
+    "paged_attention_device": (
+        C.c_int,
+        [_P, C.POINTER(_PagedBatch), _P, _SZ, _SZ, _SZ, _P, _SZ, _SZ, _P, _SZ, _SZ, C.c_float,
+         _SZ, _SZ, _P, _SZ, _SZ, _P, _SZ, _P, _ERRP],
     ),
     "cache_device_bytes": (_SZ, [_P]),
     "plan_device_bytes": (C.c_int, [C.POINTER(_Config), _SZ, _SZ, _SZ, _SZ, C.POINTER(_SZ), _ERRP]),
@@ -756,6 +800,94 @@ class RuntimeKv:
         self._b.call("runtime_decode_device", self._h, C.c_void_p(k_ptr), k_len, C.c_void_p(v_ptr),
                      v_len, C.c_void_p(q_ptr), q_len, num_q_heads, C.c_float(scale),
                      C.c_void_p(out_ptr), out_len, C.c_void_p(stream))
+
+
+# kivi_dtype (include/kivi.h)
+DTYPES = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+class PagedBatch:
+    """A ragged batch of a :class:`PagedCache` (``kivi_paged_batch``): device addresses of its int32
+    arrays ``slots`` [sequences], ``lengths`` [sequences], ``starts`` [sequences + 1] and ``pages``
+    [sequences][pages_per_sequence], and its sizes. The arrays must outlive the enqueued work."""
+
+    __slots__ = ("_c",)
+
+    def __init__(self, sequences, slots_ptr, lengths_ptr, starts_ptr, pages_ptr, pages_per_sequence,
+                 rows, max_rows=0, max_length=0):
+        self._c = _PagedBatch(sequences, slots_ptr or None, lengths_ptr or None, starts_ptr or None,
+                              pages_ptr or None, pages_per_sequence, rows, max_rows, max_length)
+
+
+class PagedCache:
+    """Quantized tokens of many sequences in a pool of pages (C-ABI extension, HIP library only):
+    ``num_pages`` pages of ``page_tokens`` tokens and ``num_slots`` full-precision windows. Rows
+    are ``dtype`` ("f32", "f16" or "bf16"). Pointers are device addresses, lengths and strides count
+    elements (stride 0: rows follow each other)."""
+
+    def __init__(self, backend, config, num_kv_heads, head_dim, dtype, page_tokens, num_pages, num_slots):
+        self._b = backend
+        h = C.c_void_p()
+        backend.call("paged_new", C.byref(config._c()), num_kv_heads, head_dim, DTYPES.get(dtype, -1),
+                     page_tokens, num_pages, num_slots, C.byref(h))
+        self._h = h
+
+    def __del__(self):
+        h = getattr(self, "_h", None)
+        if h:
+            self._b["paged_free"](h)
+            self._h = None
+
+    def config(self):
+        c = self._b["paged_config"](self._h)
+        return KiviConfig(c.bits, c.group_size, c.residual_length)
+
+    def num_kv_heads(self):
+        return self._b["paged_num_kv_heads"](self._h)
+
+    def head_dim(self):
+        return self._b["paged_head_dim"](self._h)
+
+    def dtype(self):
+        return next(k for k, v in DTYPES.items() if v == self._b["paged_dtype"](self._h))
+
+    def page_tokens(self):
+        return self._b["paged_page_tokens"](self._h)
+
+    def num_pages(self):
+        return self._b["paged_num_pages"](self._h)
+
+    def num_slots(self):
+        return self._b["paged_num_slots"](self._h)
+
+    def device_bytes(self):
+        return self._b["paged_device_bytes"](self._h)
+
+    def append_device(self, batch, k_ptr, k_len, v_ptr, v_len, k_stride=0, v_stride=0, stream=0):
+        """Appends the batch's rows behind the cached tokens of their sequences."""
+        self._b.call("paged_append_device", self._h, C.byref(batch._c), C.c_void_p(k_ptr or None), k_len,
+                     k_stride, C.c_void_p(v_ptr or None), v_len, v_stride, C.c_void_p(stream))
+
+    def read_device(self, batch, k_ptr, k_len, v_ptr, v_len, first_ptr=0, k_stride=0, v_stride=0, stream=0):
+        """Tokens ``first[i] + r`` of each sequence into its row ``r`` (no ``first``: from token 0)."""
+        self._b.call("paged_read_device", self._h, C.byref(batch._c), C.c_void_p(first_ptr or None),
+                     C.c_void_p(k_ptr or None), k_len, k_stride, C.c_void_p(v_ptr or None), v_len, v_stride,
+                     C.c_void_p(stream))
+
+    def attention_workspace_bytes(self, batch, num_q_heads):
+        out = _SZ(0)
+        self._b.call("paged_attention_workspace", self._h, C.byref(batch._c), num_q_heads, C.byref(out))
+        return out.value
+
+    def attention_device(self, batch, q_ptr, q_len, num_q_heads, scale, out_ptr, out_len, workspace_ptr,
+                         workspace_bytes, k_ptr=0, k_len=0, v_ptr=0, v_len=0, window=0, sinks=0, q_stride=0,
+                         k_stride=0, v_stride=0, out_stride=0, stream=0):
+        """Causal attention of the batch's new tokens over their sequences; without ``k_ptr`` and
+        ``v_ptr`` the new tokens are the cache's last ones."""
+        self._b.call("paged_attention_device", self._h, C.byref(batch._c), C.c_void_p(q_ptr or None), q_len,
+                     q_stride, num_q_heads, C.c_void_p(k_ptr or None), k_len, k_stride, C.c_void_p(v_ptr or None),
+                     v_len, v_stride, C.c_float(scale), window, sinks, C.c_void_p(out_ptr or None), out_len,
+                     out_stride, C.c_void_p(workspace_ptr or None), workspace_bytes, C.c_void_p(stream))
 
 
 class QualityPolicy:
