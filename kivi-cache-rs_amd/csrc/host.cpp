@@ -1620,6 +1620,9 @@ Status create_paged(const kivi_config* config, size_t heads, size_t head_dim, in
   g.pages = static_cast<uint32_t>(num_pages);
   g.slots = static_cast<uint32_t>(num_slots);
   g.type = static_cast<uint32_t>(dtype);
+  g.page_blocks = g.P / kPagedBlock;
+  g.page_magic = magic_of(g.page_blocks);
+  g.group_magic = magic_of(g.G);
   // words of a record: at most 256 tokens' worth of f32 pairs per token and channel
   size_t record, pages_bytes, rows, window_bytes;
   KIVI_TRY(mul4(page_tokens, g.DP, 32, 1, &record));

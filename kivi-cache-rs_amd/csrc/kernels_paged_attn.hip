@@ -17,15 +17,11 @@
 #include <algorithm>
 
 #include "common.hpp"
+#include "paged_attn.hpp"
 
 namespace kivi {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 // 32x32 tiles, 16 of the contraction: lane holds row (column) lane % 32, elements 8 (lane / 32) + j;
@@ -34,111 +30,30 @@ template <class T>
 struct Mma;
 template <>
 struct Mma<_Float16> {
-  typedef f16x8 Frag;
-  static __device__ __forceinline__ f32x16 mul(Frag a, Frag b, f32x16 c) {
+  static __device__ __forceinline__ f32x16 mul(f16x8 a, f16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
   }
 };
 template <>
 struct Mma<__bf16> {
-  typedef bf16x8 Frag;
-  static __device__ __forceinline__ f32x16 mul(Frag a, Frag b, f32x16 c) {
+  static __device__ __forceinline__ f32x16 mul(bf16x8 a, bf16x8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
   }
 };
 // Eight products of two: slice j takes element j of both halves, the same ones of both operands.
 template <>
 struct Mma<float> {
-  typedef f32x8 Frag;
-  static __device__ __forceinline__ f32x16 mul(Frag a, Frag b, f32x16 c) {
+  static __device__ __forceinline__ f32x16 mul(f32x8 a, f32x8 b, f32x16 c) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
     return c;
   }
 };
 
-// What a call does to one (sequence, KV head): lengths, and which tokens a tile of rows walks.
-struct Walk {
-  int64_t total;     // tokens: cached, then the new rows where they come as rows
-  int64_t hi;        // tokens from here on are seen by no row of the tile
-  int64_t lo;        // under a window, tokens in [sinks, lo) neither
-  int64_t sinks;
-  uint32_t head_tiles, first_tile, tiles;  // token tiles 0 .. head_tiles - 1, then from first_tile on; their number
+// How the chunk kernel is launched: sequences whose KV heads have more than `over` rows.
+struct ChunkPlan {
+  uint32_t over, tile_rows, tile, splits, least;
 };
-
-__device__ __forceinline__ Walk walk_of(const PagedAttention& a, const PagedSequence& s, uint32_t row0, uint32_t row1,
-                                        uint32_t gq, uint32_t tile) {
-  Walk w;
-  w.total = s.n + (a.keys.p != nullptr ? s.m : 0);
-  const int64_t p0 = w.total - s.m + row0 / gq, p1 = w.total - s.m + (row1 - 1) / gq;
-  w.hi = p1 + 1 > 0 ? p1 + 1 : 0;
-  w.lo = w.sinks = 0;
-  if (a.window != 0) {
-    w.lo = p0 + 1 > 0 && (uint64_t)(p0 + 1) > a.window ? p0 + 1 - (int64_t)a.window : 0;
-    w.sinks = (uint64_t)w.lo < a.sinks ? w.lo : (int64_t)a.sinks;
-  }
-  w.head_tiles = (uint32_t)((w.sinks + tile - 1) / tile);
-  const uint32_t from = (uint32_t)(w.lo / tile), to = (uint32_t)((w.hi + tile - 1) / tile);
-  w.first_tile = from > w.head_tiles ? from : w.head_tiles;
-  w.tiles = w.head_tiles + (to > w.first_tile ? to - w.first_tile : 0);
-  return w;
-}
-
-// Tiles [from, to) of split `split` of at most `splits`, and how many splits the walk takes (at least 1).
-struct Part {
-  uint32_t from, to, count;
-};
-constexpr uint32_t kMinTiles = 4;  // tiles that a split takes at least
-__device__ __forceinline__ Part part_of(uint32_t tiles, uint32_t splits, uint32_t split) {
-  uint32_t per = (tiles + splits - 1) / splits;
-  per = per < kMinTiles ? kMinTiles : per;
-  Part p;
-  p.count = tiles == 0 ? 1 : (tiles + per - 1) / per;
-  p.from = split * per < tiles ? split * per : tiles;
-  p.to = p.from + per < tiles ? p.from + per : tiles;
-  return p;
-}
-
-template <class T>
-__device__ __forceinline__ float decoded(uint32_t code, float2 pair) {
-  return fmaf((float)code, pair.x, pair.y);
-}
-
-// Row of token t (t >= what is packed) of one head: in the window, or among the new rows.
-template <class T>
-__device__ __forceinline__ const T* row_of(const PagedGeometry& g, const void* window, const PagedSequence& s,
-                                           uint32_t head, int64_t t, const PagedRows& rows) {
-  if (t < s.n)
-    return static_cast<const T*>(window) + (((uint64_t)s.slot * g.heads + head) * 2 * g.R + (uint64_t)t % (2 * g.R)) * g.D;
-  return static_cast<const T*>(rows.p) + (uint64_t)(s.row0 + (t - s.n)) * rows.stride + (uint64_t)head * g.D;
-}
-
-template <class T>
-__device__ __forceinline__ typename Mma<T>::Frag load_frag(const T* p, bool vec, uint32_t d, uint32_t D) {
-  typename Mma<T>::Frag f;
-  if (vec && d + 8 <= D) {
-    uint4* e = reinterpret_cast<uint4*>(&f);
-    e[0] = reinterpret_cast<const uint4*>(p + d)[0];
-    if constexpr (sizeof(T) == 4) e[1] = reinterpret_cast<const uint4*>(p + d)[1];
-  } else {
-#pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) f[j] = d + j < D ? p[d + j] : (T)0.f;
-  }
-  return f;
-}
-
-// Value (t, d) of one head, t among what the row tile walks; `rec` the record of t's page.
-template <class T>
-__device__ float value_of(const PagedAttention& a, const PagedSequence& s, const uint32_t* rec, uint32_t head, int64_t t,
-                          int64_t vq, uint32_t d) {
-  const PagedGeometry& g = a.c.geo;
-  if (t >= vq) return (float)row_of<T>(g, a.c.vwin, s, head, t, a.values)[d];
-  if (rec == nullptr) return 0.f;
-  const uint32_t in_page = (uint32_t)((uint64_t)t % g.P), tau = in_page % 32, j = tau % 4 + tau / 16 * 4;
-  const uint32_t* words = rec + g.vcodes_at() + (uint64_t)(in_page / 32) * g.block_words() + (tau % 16 / 4 * 16 + d % 16) * g.lane_words();
-  const float2 pair = reinterpret_cast<const float2*>(rec + g.vparams_at())[(uint64_t)in_page * g.ncg() + d / g.G];
-  return (float)(T)decoded<T>(words[paged_word(g.bits, d / 16, j)] >> paged_bit(g.bits, d / 16, j) & g.levels(), pair);
-}
 
 // One workgroup: WAVES * 32 rows of one (sequence, KV head), each wave 32 of them, over one split of the
 // token tiles. A tile of TT tokens lies in LDS as the products read it, keys by token, values by
@@ -146,8 +61,8 @@ __device__ float value_of(const PagedAttention& a, const PagedSequence& s, const
 // read fall on different banks. All waves fill it, from codes or from rows, and all read it.
 template <class T, int DP, int WAVES, int TT>
 __global__ void __launch_bounds__(WAVES * 64)
-    k_paged_chunk(PagedAttention a, uint32_t splits, float* partial) {
-  typedef typename Mma<T>::Frag Frag;
+    k_paged_chunk(PagedAttention a, ChunkPlan plan, float* partial) {
+  typedef typename Row<T>::Frag Frag;
   constexpr int kPad = 16 / sizeof(T), kKeyPitch = DP + kPad, kValuePitch = TT + kPad;
   constexpr uint32_t kThreads = WAVES * 64, kSub = TT / 32;
   extern __shared__ __align__(16) unsigned char lds[];
@@ -160,11 +75,12 @@ __global__ void __launch_bounds__(WAVES * 64)
   const uint32_t col = lane % 32, half = lane / 32;
   const PagedSequence s = paged_sequence(a.b, g, blockIdx.z);
   const uint32_t gq = a.qh / g.heads, rows = s.m * gq;
+  const uint32_t splits = plan.splits;
   const uint32_t tile_row = blockIdx.x / splits * (WAVES * 32), split = blockIdx.x % splits;
-  if (tile_row >= rows) return;
+  if (rows <= plan.over || tile_row >= rows) return;
   const uint32_t tile_end = tile_row + WAVES * 32 < rows ? tile_row + WAVES * 32 : rows;
   const Walk w = walk_of(a, s, tile_row, tile_end, gq, TT);
-  const Part part = part_of(w.tiles, splits, split);
+  const Part part = part_of(w.tiles, splits, plan.least, split);
   if (split >= part.count) return;
 
   const uint32_t D = g.D, S = g.S(), LW = g.lane_words(), levels = g.levels();
@@ -366,16 +282,18 @@ __global__ void __launch_bounds__(WAVES * 64)
 // Joins the splits of one row and query head per wave, its lanes over the channels.
 template <class T>
 __global__ void __launch_bounds__(256)
-    k_paged_join(PagedAttention a, uint32_t splits, uint32_t tile_rows, uint32_t tile, const float* partial) {
+    k_paged_chunk_join(PagedAttention a, ChunkPlan plan, const float* partial) {
   const PagedGeometry& g = a.c.geo;
   const PagedSequence s = paged_sequence(a.b, g, blockIdx.z);
   const uint32_t gq = a.qh / g.heads, rows = s.m * gq, lane = threadIdx.x % 64;
+  const uint32_t splits = plan.splits, tile_rows = plan.tile_rows;
+  if (rows <= plan.over) return;
   const uint64_t all = (uint64_t)a.b.rows * a.qh;
   for (uint64_t i = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64; i < (uint64_t)s.m * a.qh; i += (uint64_t)gridDim.x * 4) {
     const uint32_t token = (uint32_t)(i / a.qh), qhead = (uint32_t)(i % a.qh), r = token * gq + qhead % gq;
     const uint32_t r0 = r / tile_rows * tile_rows;
-    const Walk w = walk_of(a, s, r0, r0 + tile_rows < rows ? r0 + tile_rows : rows, gq, tile);
-    const uint32_t count = part_of(w.tiles, splits, 0).count;
+    const Walk w = walk_of(a, s, r0, r0 + tile_rows < rows ? r0 + tile_rows : rows, gq, plan.tile);
+    const uint32_t count = part_of(w.tiles, splits, plan.least, 0).count;
     if (count == 1) continue;
     const uint64_t place = (uint64_t)s.row0 * a.qh + i;
     const float2* state = reinterpret_cast<const float2*>(partial + splits * all * g.DP);
@@ -399,60 +317,118 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-// How a call is cut: rows of a workgroup, tokens of a tile, splits.
+// How a call is cut. The lengths are device memory, so the plan goes by the host's bounds: sequences
+// shorter than those take fewer of the planned splits, and their other workgroups end at once.
 struct Plan {
-  uint32_t waves, tile, splits;
+  RowsPlan rows[2];
+  uint32_t row_launches;
+  bool chunks;
+  ChunkPlan chunk;
+  size_t rows_at[2], chunk_at, floats;  // the launches' partials in the workspace
 };
 
-constexpr uint32_t kTargetWorkgroups = 1024;  // four per compute unit
+// Workgroups that the longest lengths would give: many more than run at once (256 compute units, two or
+// so each), so that ragged lengths even out.
+constexpr uint64_t kRowsWorkgroups = 8192;
+constexpr uint64_t kChunkWorkgroups = 1024;
+constexpr uint64_t kMostSplits = 512;
 
-Plan plan_of(const PagedGeometry& g, const PagedBatch& b, uint32_t qh) {
-  Plan p;
-  const uint64_t rows = (uint64_t)b.max_rows * (qh / g.heads);
-  p.waves = 4;
-  p.tile = g.type == kPagedF32 && g.DP > 128 ? 32 : 64;
-  const uint64_t groups = (rows + p.waves * 32 - 1) / (p.waves * 32) * g.heads * b.sequences;
-  const uint64_t tiles = (b.max_length + b.max_rows + p.tile - 1) / p.tile;
-  const uint64_t most = std::max<uint64_t>(1, tiles / kMinTiles);
-  const uint64_t want = groups == 0 ? 1 : (kTargetWorkgroups + groups - 1) / groups;
-  p.splits = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({want, most, 64}));
+Plan plan_of(const PagedGeometry& g, const PagedBatch& b, uint32_t qh, uint64_t window, uint64_t sinks) {
+  Plan p{};
+  const uint32_t gq = qh / g.heads;
+  const uint64_t rows = (uint64_t)b.max_rows * gq;
+  // the workspace is sized without a window, which only ever walks less
+  const uint64_t all = b.max_length + b.max_rows;
+  const uint64_t tokens =
+      window == 0 ? all : std::min(all, window + std::min(sinks, all) + b.max_rows + 2 * kPagedBlock);
+  const uint64_t heads = (uint64_t)b.sequences * g.heads;
+  if (paged_rows_take(g)) {
+    // One launch for what a decoded token brings (gq rows), one for more rows than its tiles hold.
+    const uint32_t decode = gq <= 4 ? 4 : gq <= 8 ? 8 : kRowsMost;
+    const uint32_t most[2] = {decode, kRowsMost};
+    uint32_t over = 0;
+    for (uint32_t i = 0; i < 2 && over < rows && over < kRowsMost; ++i) {
+      RowsPlan& r = p.rows[p.row_launches];
+      r.over = over;
+      r.most = most[i];
+      r.stride = (uint32_t)std::min<uint64_t>(rows, r.most);
+      r.blocks = r.stride <= 4 ? 4 : r.stride <= 8 ? 2 : 1;
+      const uint64_t turn = 4 * r.blocks, tiles = (r.stride + 16 / r.blocks - 1) / (16 / r.blocks);
+      // blocks of a split and the splits of a walk over n tokens, at most `cap`
+      const auto cut = [&](uint64_t n, uint64_t cap) {
+        const uint64_t blocks = std::max<uint64_t>(1, (n + kPagedBlock - 1) / kPagedBlock);
+        const uint64_t least = std::max(blocks * heads * tiles / kRowsWorkgroups, (blocks + cap - 1) / cap);
+        r.least = (uint32_t)((std::max<uint64_t>(1, least) + turn - 1) / turn * turn);
+        r.splits = (uint32_t)((blocks + r.least - 1) / r.least);
+      };
+      cut(all, kMostSplits);
+      const uint64_t most_splits = r.splits;
+      if (tokens < all) cut(tokens, most_splits);
+      p.rows_at[p.row_launches++] = p.floats;
+      p.floats += heads * r.stride * (most_splits + 1) * (g.DP + 2);  // and the last blocks
+      over = most[i];
+    }
+    p.chunk.over = kRowsMost;
+  }
+  p.chunks = rows > p.chunk.over;
+  p.chunk.tile_rows = 128;
+  p.chunk.tile = g.type == kPagedF32 && g.DP > 128 ? 32 : 64;
+  p.chunk.least = 4;
+  const uint64_t groups = std::max<uint64_t>(1, (uint64_t)b.rows * gq / p.chunk.tile_rows) * g.heads;
+  const uint64_t want = std::min<uint64_t>((kChunkWorkgroups + groups - 1) / groups, 64);
+  const auto chunk_splits = [&](uint64_t n) {
+    return (uint32_t)std::max<uint64_t>(1, std::min(want, (n + p.chunk.tile - 1) / p.chunk.tile / p.chunk.least));
+  };
+  p.chunk.splits = chunk_splits(tokens);
+  p.chunk_at = p.floats;
+  if (p.chunks && chunk_splits(all) > 1) p.floats += (size_t)chunk_splits(all) * (size_t)b.rows * qh * (g.DP + 2);
   return p;
 }
 
 template <class T, int DP>
-hipError_t chunk_typed(const PagedAttention& a, float* workspace, hipStream_t stream) {
+hipError_t launch_chunk(const PagedAttention& a, const ChunkPlan& p, float* partial, hipStream_t stream) {
   constexpr int WAVES = 4, TT = sizeof(T) == 4 && DP > 128 ? 32 : 64, kPad = 16 / sizeof(T);
   const PagedGeometry& g = a.c.geo;
-  const Plan p = plan_of(g, a.b, a.qh);
   const uint64_t rows = (uint64_t)a.b.max_rows * (a.qh / g.heads);
   const uint64_t x = (rows + WAVES * 32 - 1) / (WAVES * 32) * p.splits;
   const size_t bytes = (TT * (DP + kPad) + DP * (TT + kPad)) * sizeof(T);
   auto kernel = k_paged_chunk<T, DP, WAVES, TT>;
   hipError_t e = raise_lds_limit(reinterpret_cast<const void*>(kernel), bytes);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(kernel, dim3((uint32_t)x, g.heads, a.b.sequences), dim3(WAVES * 64), bytes, stream, a, p.splits, workspace);
+  hipLaunchKernelGGL(kernel, dim3((uint32_t)x, g.heads, a.b.sequences), dim3(WAVES * 64), bytes, stream, a, p, partial);
   if (p.splits > 1) {
     const uint64_t joins = std::min<uint64_t>(((uint64_t)a.b.max_rows * a.qh + 3) / 4, 1u << 16);
-    hipLaunchKernelGGL(k_paged_join<T>, dim3((uint32_t)joins, 1, a.b.sequences), dim3(256), 0, stream, a, p.splits, WAVES * 32u,
-                       (uint32_t)TT, workspace);
+    hipLaunchKernelGGL(k_paged_chunk_join<T>, dim3((uint32_t)joins, 1, a.b.sequences), dim3(256), 0, stream, a, p, partial);
   }
   return hipGetLastError();
 }
 
 template <class T>
 hipError_t attention_typed(const PagedAttention& a, float* workspace, hipStream_t stream) {
+  const Plan p = plan_of(a.c.geo, a.b, a.qh, a.window, a.sinks);
+  for (uint32_t i = 0; i < p.row_launches; ++i) {
+    const hipError_t e = launch_paged_rows<T>(a, p.rows[i], workspace + p.rows_at[i], stream);
+    if (e != hipSuccess) return e;
+  }
+  if (!p.chunks) return hipSuccess;
   const uint32_t DP = a.c.geo.DP;
-  if (DP <= 64) return chunk_typed<T, 64>(a, workspace, stream);
-  if (DP <= 96) return chunk_typed<T, 96>(a, workspace, stream);
-  if (DP <= 128) return chunk_typed<T, 128>(a, workspace, stream);
-  return chunk_typed<T, 256>(a, workspace, stream);
+  float* partial = workspace + p.chunk_at;
+  if (DP <= 64) return launch_chunk<T, 64>(a, p.chunk, partial, stream);
+  if (DP <= 96) return launch_chunk<T, 96>(a, p.chunk, partial, stream);
+  if (DP <= 128) return launch_chunk<T, 128>(a, p.chunk, partial, stream);
+  return launch_chunk<T, 256>(a, p.chunk, partial, stream);
 }
 
 }  // namespace
 
+// The kernel of few rows scales one 16-token tile by one group's pairs, and a wave reads whole words.
+bool paged_rows_take(const PagedGeometry& g) {
+  const uint32_t S = g.S();
+  return g.G % 16 == 0 && (S == 2 || S == 3 || S == 4 || S == 8);
+}
+
 size_t paged_attention_workspace(const PagedGeometry& g, const PagedBatch& b, uint32_t qh) {
-  const Plan p = plan_of(g, b, qh);
-  return p.splits == 1 ? 0 : (size_t)p.splits * (size_t)b.rows * qh * (g.DP + 2) * sizeof(float);
+  return plan_of(g, b, qh, 0, 0).floats * sizeof(float);
 }
 
 hipError_t launch_paged_attention(const PagedAttention& a, float* workspace, hipStream_t stream) {

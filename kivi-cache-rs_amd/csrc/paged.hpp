@@ -44,6 +44,14 @@ constexpr uint32_t kPagedMaxSpan = 512;    // lcm(32, G): tokens a key-quantizin
 
 enum PagedType : uint32_t { kPagedF32 = 0, kPagedF16 = 1, kPagedBF16 = 2 };
 
+// n / d by a multiplication, any n and d: magic_of(d) falls short of 2^32 / d by less than one (two for d =
+// 1), so the estimate falls short of the quotient by at most one.
+__host__ inline uint32_t magic_of(uint32_t d) { return d == 1 ? 0xffffffffu : (uint32_t)(((uint64_t)1 << 32) / d); }
+__device__ __forceinline__ uint32_t quotient(uint32_t n, uint32_t d, uint32_t magic) {
+  const uint32_t e = __umulhi(n, magic);
+  return n - e * d >= d ? e + 1 : e;
+}
+
 struct PagedGeometry {
   uint32_t bits, G, R, D, DP;
   uint32_t heads;
@@ -52,6 +60,8 @@ struct PagedGeometry {
   uint32_t pages;  // pages of the pool
   uint32_t slots;  // windows
   uint32_t type;   // PagedType
+  uint32_t page_blocks;  // P / 32
+  uint32_t page_magic, group_magic;  // magic_of(page_blocks), magic_of(G)
 
   __host__ __device__ uint32_t S() const { return DP / 32; }
   __host__ __device__ uint32_t ncg() const { return D / G; }
@@ -111,14 +121,19 @@ __device__ __forceinline__ PagedSequence paged_sequence(const PagedBatch& b, con
   return s;
 }
 
-// Record of (page of token t, head), or null where the sequence has no such page.
-__device__ __forceinline__ uint32_t* paged_record(const PagedView& c, const PagedBatch& b, const PagedSequence& s,
-                                                  uint32_t head, int64_t t) {
-  const uint64_t p = (uint64_t)t / c.geo.P;
+// Record of (the sequence's page p, head), or null where it has no such page.
+__device__ __forceinline__ uint32_t* paged_record_of(const PagedView& c, const PagedBatch& b, const PagedSequence& s,
+                                                     uint32_t head, uint32_t p) {
   if (p >= b.per_sequence) return nullptr;
   const int32_t page = s.table[p];
   if (page < 0 || (uint32_t)page >= c.geo.pages) return nullptr;
   return c.pages + ((uint64_t)(uint32_t)page * c.geo.heads + head) * c.geo.record_words();
+}
+
+// The same of the page of token t.
+__device__ __forceinline__ uint32_t* paged_record(const PagedView& c, const PagedBatch& b, const PagedSequence& s,
+                                                  uint32_t head, int64_t t) {
+  return paged_record_of(c, b, s, head, quotient((uint32_t)(t / kPagedBlock), c.geo.page_blocks, c.geo.page_magic));
 }
 
 __host__ __device__ inline int64_t paged_kq(const PagedGeometry& g, int64_t n) { return n / g.R * g.R; }

@@ -1,0 +1,132 @@
+// paged_attn.hpp — what the attention kernels of the paged cache share: which tokens a tile of rows
+// walks, how a walk is split, where a token's row lies, and the launches of the two kernels.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include "paged.hpp"
+
+namespace kivi {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLargest = 3.402823466e+38f;  // |x| <= kLargest: x is finite
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+// Eight elements of a row.
+template <class T>
+struct Row;
+template <>
+struct Row<_Float16> {
+  typedef f16x8 Frag;
+};
+template <>
+struct Row<__bf16> {
+  typedef bf16x8 Frag;
+};
+template <>
+struct Row<float> {
+  typedef f32x8 Frag;
+};
+
+// What a call does to one (sequence, KV head): lengths, and which tokens a tile of rows walks.
+struct Walk {
+  int64_t total;     // tokens: cached, then the new rows where they come as rows
+  int64_t hi;        // tokens from here on are seen by no row of the tile
+  int64_t lo;        // under a window, tokens in [sinks, lo) neither
+  int64_t sinks;
+  uint32_t head_tiles, first_tile, tiles;  // token tiles 0 .. head_tiles - 1, then from first_tile on; their number
+};
+
+__device__ __forceinline__ Walk walk_of(const PagedAttention& a, const PagedSequence& s, uint32_t row0, uint32_t row1,
+                                        uint32_t gq, uint32_t tile) {
+  Walk w;
+  w.total = s.n + (a.keys.p != nullptr ? s.m : 0);
+  const int64_t p0 = w.total - s.m + row0 / gq, p1 = w.total - s.m + (row1 - 1) / gq;
+  w.hi = p1 + 1 > 0 ? p1 + 1 : 0;
+  w.lo = w.sinks = 0;
+  if (a.window != 0) {
+    w.lo = p0 + 1 > 0 && (uint64_t)(p0 + 1) > a.window ? p0 + 1 - (int64_t)a.window : 0;
+    w.sinks = (uint64_t)w.lo < a.sinks ? w.lo : (int64_t)a.sinks;
+  }
+  w.head_tiles = (uint32_t)((w.sinks + tile - 1) / tile);
+  const uint32_t from = (uint32_t)(w.lo / tile), to = (uint32_t)((w.hi + tile - 1) / tile);
+  w.first_tile = from > w.head_tiles ? from : w.head_tiles;
+  w.tiles = w.head_tiles + (to > w.first_tile ? to - w.first_tile : 0);
+  return w;
+}
+
+// Tiles [from, to) of split `split` of at most `splits`, each a multiple of `least` tiles, and how many
+// splits the walk takes (at least 1).
+struct Part {
+  uint32_t from, to, count;
+};
+__device__ __forceinline__ Part part_of(uint32_t tiles, uint32_t splits, uint32_t least, uint32_t split) {
+  uint32_t per = (tiles + splits - 1) / splits;
+  per = (per + least - 1) / least * least;
+  Part p;
+  p.count = tiles == 0 ? 1 : (tiles + per - 1) / per;
+  p.from = split * per < tiles ? split * per : tiles;
+  p.to = p.from + per < tiles ? p.from + per : tiles;
+  return p;
+}
+
+template <class T>
+__device__ __forceinline__ float decoded(uint32_t code, float2 pair) {
+  return fmaf((float)code, pair.x, pair.y);
+}
+
+// Row of token t (t >= what is packed) of one head: in the window, or among the new rows.
+template <class T>
+__device__ __forceinline__ const T* row_of(const PagedGeometry& g, const void* window, const PagedSequence& s,
+                                           uint32_t head, int64_t t, const PagedRows& rows) {
+  if (t < s.n)
+    return static_cast<const T*>(window) + (((uint64_t)s.slot * g.heads + head) * 2 * g.R + (uint64_t)t % (2 * g.R)) * g.D;
+  return static_cast<const T*>(rows.p) + (uint64_t)(s.row0 + (t - s.n)) * rows.stride + (uint64_t)head * g.D;
+}
+
+template <class T>
+__device__ __forceinline__ typename Row<T>::Frag load_frag(const T* p, bool vec, uint32_t d, uint32_t D) {
+  typename Row<T>::Frag f;
+  if (vec && d + 8 <= D) {
+    uint4* e = reinterpret_cast<uint4*>(&f);
+    e[0] = reinterpret_cast<const uint4*>(p + d)[0];
+    if constexpr (sizeof(T) == 4) e[1] = reinterpret_cast<const uint4*>(p + d)[1];
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 8; ++j) f[j] = d + j < D ? p[d + j] : (T)0.f;
+  }
+  return f;
+}
+
+// Value (t, d) of one head, t among what the row tile walks; `rec` the record of t's page.
+template <class T>
+__device__ float value_of(const PagedAttention& a, const PagedSequence& s, const uint32_t* rec, uint32_t head, int64_t t,
+                          int64_t vq, uint32_t d) {
+  const PagedGeometry& g = a.c.geo;
+  if (t >= vq) return (float)row_of<T>(g, a.c.vwin, s, head, t, a.values)[d];
+  if (rec == nullptr) return 0.f;
+  const uint32_t in_page = (uint32_t)((uint64_t)t % g.P), tau = in_page % 32, j = tau % 4 + tau / 16 * 4;
+  const uint32_t* words = rec + g.vcodes_at() + (uint64_t)(in_page / 32) * g.block_words() + (tau % 16 / 4 * 16 + d % 16) * g.lane_words();
+  const float2 pair = reinterpret_cast<const float2*>(rec + g.vparams_at())[(uint64_t)in_page * g.ncg() + d / g.G];
+  return (float)(T)decoded<T>(words[paged_word(g.bits, d / 16, j)] >> paged_bit(g.bits, d / 16, j) & g.levels(), pair);
+}
+
+// Chunks of few rows (kernels_paged_rows_*.hip): sequences whose KV heads have more than `over` and at
+// most `most` rows, at most kRowsMost.
+constexpr uint32_t kRowsMost = 32;
+struct RowsPlan {
+  uint32_t over, most;     // rows of a KV head that this launch takes
+  uint32_t blocks;         // column groups: 4 (up to 4 rows), 2 (8) or 1 (16 rows a tile)
+  uint32_t splits;         // at most this many of a walk,
+  uint32_t least;          // each of a multiple of this many 32-token blocks (itself one of 4 * blocks)
+  uint32_t stride;         // rows of a (sequence, head) in the partials
+};
+// Whether the kernels of few rows take this cache (else the chunk kernel takes everything).
+bool paged_rows_take(const PagedGeometry& g);
+template <class T>
+hipError_t launch_paged_rows(const PagedAttention& a, const RowsPlan& p, float* partial, hipStream_t stream);
+
+}  // namespace kivi
