@@ -1620,14 +1620,12 @@ Status create_paged(const kivi_config* config, size_t heads, size_t head_dim, in
   g.pages = static_cast<uint32_t>(num_pages);
   g.slots = static_cast<uint32_t>(num_slots);
   g.type = static_cast<uint32_t>(dtype);
-  g.page_blocks = g.P / kPagedBlock;
-  g.page_magic = magic_of(g.page_blocks);
-  g.group_magic = magic_of(g.G);
-  // words of a record: at most 256 tokens' worth of f32 pairs per token and channel
+  // a record's words are counted in 32 bits: 32 a token and channel are more than it ever has
   size_t record, pages_bytes, rows, window_bytes;
   KIVI_TRY(mul4(page_tokens, g.DP, 32, 1, &record));
   if (record > UINT32_MAX) return Err(KIVI_ERR_UNSUPPORTED, page_tokens, UINT32_MAX / (32 * g.DP), "page_tokens");
-  KIVI_TRY(mul4(num_pages, heads, g.record_words(), 4, &pages_bytes));
+  g.finish();
+  KIVI_TRY(mul4(num_pages, heads, g.record_words, 4, &pages_bytes));
   KIVI_TRY(mul4(num_slots, heads, 2 * config->residual_length, 1, &rows));
   KIVI_TRY(mul4(rows, head_dim, g.type_bytes(), 1, &window_bytes));
   c->cfg = *config;

@@ -68,7 +68,7 @@ template <class T>
 __device__ __forceinline__ const T* token_row(const PagedGeometry& g, const T* window, const PagedSequence& s,
                                               uint32_t head, int64_t t, const T* rows, uint64_t stride) {
   if (t < s.n)
-    return window + (((uint64_t)s.slot * g.heads + head) * 2 * g.R + (uint64_t)t % (2 * g.R)) * g.D;
+    return window + (((uint64_t)s.slot * g.heads + head) * 2 * g.R + ring_row(g, t)) * g.D;
   return rows + (uint64_t)(s.row0 + (t - s.n)) * stride + (uint64_t)head * g.D;
 }
 
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kThreads)
     }
     __syncthreads();
     const uint32_t g0 = (uint32_t)(lo - base) / g.G, ng = count / g.G;
-    float2* params = reinterpret_cast<float2*>(rec + g.kparams_at()) + (uint64_t)((uint64_t)base % g.P / g.G) * g.DP;
+    float2* params = reinterpret_cast<float2*>(rec + g.kparams_at) + (uint64_t)quotient(token_in_page(g, base), g.G, g.group_magic) * g.DP;
     for (uint32_t i = tid / kReduce; i < ng * CH; i += kThreads / kReduce) {
       const uint32_t gi = g0 + i / CH, ch = i % CH;
       const float2 p = group_pair(tile + gi * g.G * pitch + ch, pitch, g.G, flevels);
@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(kThreads)
       }
     }
     __syncthreads();
-    uint32_t* codes = rec + (uint64_t)base % g.P / kPagedBlock * g.block_words();
+    uint32_t* codes = rec + (uint64_t)(token_in_page(g, base) / kPagedBlock) * g.block_words();
     for (uint32_t i = tid; i < g.span / kPagedBlock * 16 * LW; i += kThreads) {
       const uint32_t w = i % LW, l = i / LW % 16, blk = i / LW / 16;
       uint32_t word = 0, mask = 0;
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kThreads)
     if (lo >= hi) return;
     uint32_t* rec = paged_record(c, b, s, head, base);
     if (rec == nullptr) return;
-    const uint32_t pitch = g.DP + 1, ncg = g.ncg(), oct = g.DP / 8;
+    const uint32_t pitch = g.DP + 1, ncg = g.ncg, oct = g.DP / 8;
     float* tile = lds;                                                              // [32][pitch]
     float2* pair = reinterpret_cast<float2*>(lds + ((kPagedBlock * pitch + 1) & ~1u));  // [32][ncg]
     const uint32_t t0 = (uint32_t)(lo - base), count = (uint32_t)(hi - lo);
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(kThreads)
       for (uint32_t j = 0; j < 8; ++j) tile[(uint32_t)(t - base) * pitch + d + j] = x[j];
     }
     __syncthreads();
-    float2* params = reinterpret_cast<float2*>(rec + g.vparams_at()) + (uint64_t)base % g.P * ncg;
+    float2* params = reinterpret_cast<float2*>(rec + g.vparams_at) + (uint64_t)token_in_page(g, base) * ncg;
     for (uint32_t i = tid / kReduce; i < count * ncg; i += kThreads / kReduce) {
       const uint32_t tau = t0 + i / ncg, cg = i % ncg;
       const float2 p = group_pair(tile + tau * pitch + cg * g.G, 1, g.G, flevels);
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kThreads)
       }
     }
     __syncthreads();
-    uint32_t* codes = rec + g.vcodes_at() + (uint64_t)base % g.P / kPagedBlock * g.block_words();
+    uint32_t* codes = rec + g.vcodes_at + (uint64_t)(token_in_page(g, base) / kPagedBlock) * g.block_words();
     for (uint32_t i = tid; i < 64 * LW; i += kThreads) {
       const uint32_t w = i % LW, lane = i / LW, q = lane / 16, l = lane % 16;
       uint32_t word = 0, mask = 0;
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kThreads)
   for (int64_t i = tid; lo + i / D < hi; i += kThreads) {
     const int64_t t = lo + i / D;
     const uint32_t d = (uint32_t)(i % D);
-    const uint64_t to = (((uint64_t)s.slot * g.heads + head) * 2 * g.R + (uint64_t)t % (2 * g.R)) * D + d;
+    const uint64_t to = (((uint64_t)s.slot * g.heads + head) * 2 * g.R + ring_row(g, t)) * D + d;
     const uint64_t row = (uint64_t)(s.row0 + (t - n));
     static_cast<T*>(c.kwin)[to] = kr[row * keys.stride + (uint64_t)head * D + d];
     static_cast<T*>(c.vwin)[to] = vr[row * values.stride + (uint64_t)head * D + d];
@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(kThreads)
   if (s.m == 0) return;
   const int32_t from = first != nullptr ? first[blockIdx.z] : 0;
   const int64_t f0 = from > 0 ? from : 0, end = f0 + s.m, n = s.n;
-  const uint32_t D = g.D, S = g.S(), LW = g.lane_words(), levels = g.levels(), oct = (D + 7) / 8, ncg = g.ncg();
+  const uint32_t D = g.D, S = g.S(), LW = g.lane_words(), levels = g.levels(), oct = (D + 7) / 8, ncg = g.ncg;
   const bool wvec = D * sizeof(T) % 16 == 0;
   const T* kw = static_cast<const T*>(c.kwin);
   const T* vw = static_cast<const T*>(c.vwin);
@@ -268,10 +268,10 @@ __global__ void __launch_bounds__(kThreads)
     const int64_t base = blk * kPagedBlock;
     const int64_t lo = base > f0 ? base : f0, hi = base + kPagedBlock < end ? base + kPagedBlock : end;
     const uint32_t* rec = base < n ? paged_record(c, b, s, head, base) : nullptr;
-    const uint32_t in_page = (uint32_t)((uint64_t)base % g.P);
+    const uint32_t in_page = token_in_page(g, base);
     if (base < vq && rec != nullptr) {
-      const uint32_t* codes = rec + g.vcodes_at() + (uint64_t)(in_page / kPagedBlock) * g.block_words();
-      const float2* pairs = reinterpret_cast<const float2*>(rec + g.vparams_at()) + (uint64_t)in_page * ncg;
+      const uint32_t* codes = rec + g.vcodes_at + (uint64_t)(in_page / kPagedBlock) * g.block_words();
+      const float2* pairs = reinterpret_cast<const float2*>(rec + g.vparams_at) + (uint64_t)in_page * ncg;
       for (uint32_t i = tid; i < 64 * 2 * S; i += kThreads) {
         const uint32_t lane = i % 64, f = i / 64, d = 16 * f + lane % 16, q = lane / 16;
         if (d >= D) continue;
@@ -296,7 +296,7 @@ __global__ void __launch_bounds__(kThreads)
           const uint32_t q = d / (8 * S), f = tau / 16 * S + d % (8 * S) / 8;
           const uint32_t* words = codes + (q * 16 + tau % 16) * LW;
           const float2* pairs =
-              reinterpret_cast<const float2*>(rec + g.kparams_at()) + (uint64_t)((in_page + tau) / g.G) * g.DP + d;
+              reinterpret_cast<const float2*>(rec + g.kparams_at) + (uint64_t)((in_page + tau) / g.G) * g.DP + d;
 #pragma unroll
           for (uint32_t j = 0; j < 8; ++j)
             x[j] = decoded(words[paged_word(g.bits, f, j)] >> paged_bit(g.bits, f, j) & levels, pairs[j]);
@@ -331,7 +331,7 @@ hipError_t append_typed(const PagedView& c, const PagedBatch& b, const PagedRows
   const uint32_t window_items = (std::min<uint64_t>(b.max_rows, g.R) + kWindowRows - 1) / kWindowRows;
   const uint32_t ch = 8 * g.S();
   const size_t key_lds = ((g.span * (ch + 1) + 1) & ~1u) * 4ull + (uint64_t)g.span / g.G * ch * 8;
-  const size_t value_lds = ((kPagedBlock * (g.DP + 1) + 1) & ~1u) * 4ull + (uint64_t)kPagedBlock * g.ncg() * 8;
+  const size_t value_lds = ((kPagedBlock * (g.DP + 1) + 1) & ~1u) * 4ull + (uint64_t)kPagedBlock * g.ncg * 8;
   const size_t bytes = std::max(key_lds, value_lds);
   hipError_t e = raise_lds_limit(reinterpret_cast<const void*>(&k_paged_append<T>), bytes);
   if (e != hipSuccess) return e;

@@ -103,7 +103,12 @@ __global__ void __launch_bounds__(WAVES * 64)
   {
     const T* p = static_cast<const T*>(a.query.p) + (uint64_t)(s.row0 + token) * a.query.stride + (uint64_t)qhead * D;
 #pragma unroll
-    for (int i = 0; i < DP / 16; ++i) q[i] = load_frag(p, a.query.vec != 0, 16 * i + 8 * half, D);
+    for (int i = 0; i < DP / 16; ++i) {
+      const uint32_t d = 16 * i + 8 * half;
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) q[i][j] = (T)0.f;
+      if (d < D) q[i] = load_frag(p, a.query.vec != 0, d, D);
+    }
   }
   const float scale = a.scale * kLog2e;
   float top = -INFINITY, sum = 0.f;
@@ -133,9 +138,9 @@ __global__ void __launch_bounds__(WAVES * 64)
       if (t < kq) {
         const uint32_t* r = rec[tau / 32];
         if (r != nullptr && d < g.DP) {  // DP may be more than the cache's
-          const uint32_t in_page = (uint32_t)((uint64_t)t % g.P), frag = in_page % 32 / 16 * S + o % S;
+          const uint32_t in_page = token_in_page(g, t), frag = in_page % 32 / 16 * S + o % S;
           const uint32_t* words = r + (uint64_t)(in_page / 32) * g.block_words() + (o / S * 16 + l) * LW;
-          const float2* pairs = reinterpret_cast<const float2*>(r + g.kparams_at()) + (uint64_t)(in_page / g.G) * g.DP + d;
+          const float2* pairs = reinterpret_cast<const float2*>(r + g.kparams_at) + (uint64_t)(in_page / g.G) * g.DP + d;
 #pragma unroll
           for (uint32_t j = 0; j < 8; ++j)
             f[j] = (T)decoded<T>(words[paged_word(g.bits, frag, j)] >> paged_bit(g.bits, frag, j) & levels, pairs[j]);
@@ -143,7 +148,7 @@ __global__ void __launch_bounds__(WAVES * 64)
 #pragma unroll
           for (uint32_t j = 0; j < 8; ++j) f[j] = (T)0.f;
         }
-      } else if (t < w.hi) {
+      } else if (t < w.hi && d < D) {
         f = load_frag(row_of<T>(g, a.c.kwin, s, head, t, a.keys), t < s.n ? wvec : a.keys.vec != 0, d, D);
       } else {
 #pragma unroll
@@ -352,7 +357,7 @@ Plan plan_of(const PagedGeometry& g, const PagedBatch& b, uint32_t qh, uint64_t 
       r.over = over;
       r.most = most[i];
       r.stride = (uint32_t)std::min<uint64_t>(rows, r.most);
-      r.blocks = r.stride <= 4 ? 4 : r.stride <= 8 ? 2 : 1;
+      r.blocks = std::min<uint32_t>(r.stride <= 4 ? 4 : r.stride <= 8 ? 2 : 1, rows_most_blocks(g.bits, g.S()));
       const uint64_t turn = 4 * r.blocks, tiles = (r.stride + 16 / r.blocks - 1) / (16 / r.blocks);
       // blocks of a split and the splits of a walk over n tokens, at most `cap`
       const auto cut = [&](uint64_t n, uint64_t cap) {
@@ -407,7 +412,8 @@ template <class T>
 hipError_t attention_typed(const PagedAttention& a, float* workspace, hipStream_t stream) {
   const Plan p = plan_of(a.c.geo, a.b, a.qh, a.window, a.sinks);
   for (uint32_t i = 0; i < p.row_launches; ++i) {
-    const hipError_t e = launch_paged_rows<T>(a, p.rows[i], workspace + p.rows_at[i], stream);
+    const hipError_t e = a.c.geo.G % 32 != 0 ? launch_paged_rows<T, true>(a, p.rows[i], workspace + p.rows_at[i], stream)
+                                             : launch_paged_rows<T, false>(a, p.rows[i], workspace + p.rows_at[i], stream);
     if (e != hipSuccess) return e;
   }
   if (!p.chunks) return hipSuccess;

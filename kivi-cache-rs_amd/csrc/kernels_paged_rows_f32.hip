@@ -1,8 +1,9 @@
-// kernels_paged_rows_f32.hip — attention of few rows over the paged cache, rows of f32 (paged_rows.hpp).
+// kernels_paged_rows_f32.hip — attention of few rows over the paged cache, rows of f32
+// (paged_rows.hpp).
 #include "paged_rows.hpp"
 
 namespace kivi {
 
-template hipError_t launch_paged_rows<float>(const PagedAttention&, const RowsPlan&, float*, hipStream_t);
+template hipError_t launch_paged_rows<float, false>(const PagedAttention&, const RowsPlan&, float*, hipStream_t);
 
 }  // namespace kivi

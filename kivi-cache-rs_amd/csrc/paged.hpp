@@ -60,20 +60,28 @@ struct PagedGeometry {
   uint32_t pages;  // pages of the pool
   uint32_t slots;  // windows
   uint32_t type;   // PagedType
-  uint32_t page_blocks;  // P / 32
-  uint32_t page_magic, group_magic;  // magic_of(page_blocks), magic_of(G)
+  // what follows from those (finish); offsets in words from a record
+  uint32_t ncg, page_blocks;
+  uint32_t kparams_at, vcodes_at, vparams_at, record_words;
+  uint32_t page_magic, group_magic, fragment_magic, flush_magic, ring_magic;  // of P/32, G, max(1, G/16), R, 2R
 
+  __host__ void finish() {
+    ncg = D / G;
+    page_blocks = P / kPagedBlock;
+    kparams_at = page_blocks * block_words();
+    vcodes_at = kparams_at + P / G * DP * 2;
+    vparams_at = vcodes_at + page_blocks * block_words();
+    record_words = vparams_at + P * ncg * 2;
+    page_magic = magic_of(page_blocks);
+    group_magic = magic_of(G);
+    fragment_magic = magic_of(G < 16 ? 1 : G / 16);
+    flush_magic = magic_of(R);
+    ring_magic = magic_of(2 * R);
+  }
   __host__ __device__ uint32_t S() const { return DP / 32; }
-  __host__ __device__ uint32_t ncg() const { return D / G; }
   __host__ __device__ uint32_t levels() const { return (1u << bits) - 1u; }
   __host__ __device__ uint32_t lane_words() const { return DP / 32 * bits / 2; }
   __host__ __device__ uint32_t block_words() const { return DP * bits; }  // 32 tokens * DP * bits / 32
-  __host__ __device__ uint32_t kparams_at() const { return P / 32 * block_words(); }  // in words, from the record
-  __host__ __device__ uint32_t vcodes_at() const { return kparams_at() + P / G * DP * 2; }
-  __host__ __device__ uint32_t vparams_at() const { return vcodes_at() + P / 32 * block_words(); }
-  __host__ __device__ uint32_t record_words() const { return vparams_at() + P * ncg() * 2; }
-  __host__ __device__ uint64_t page_words() const { return (uint64_t)heads * record_words(); }
-  __host__ __device__ uint64_t window_rows() const { return (uint64_t)slots * heads * 2 * R; }
   __host__ __device__ uint32_t type_bytes() const { return type == kPagedF32 ? 4u : 2u; }
 };
 
@@ -127,7 +135,7 @@ __device__ __forceinline__ uint32_t* paged_record_of(const PagedView& c, const P
   if (p >= b.per_sequence) return nullptr;
   const int32_t page = s.table[p];
   if (page < 0 || (uint32_t)page >= c.geo.pages) return nullptr;
-  return c.pages + ((uint64_t)(uint32_t)page * c.geo.heads + head) * c.geo.record_words();
+  return c.pages + ((uint64_t)(uint32_t)page * c.geo.heads + head) * c.geo.record_words;
 }
 
 // The same of the page of token t.
@@ -136,8 +144,20 @@ __device__ __forceinline__ uint32_t* paged_record(const PagedView& c, const Page
   return paged_record_of(c, b, s, head, quotient((uint32_t)(t / kPagedBlock), c.geo.page_blocks, c.geo.page_magic));
 }
 
-__host__ __device__ inline int64_t paged_kq(const PagedGeometry& g, int64_t n) { return n / g.R * g.R; }
-__host__ __device__ inline int64_t paged_vq(const PagedGeometry& g, int64_t n) { return n > g.R ? n - g.R : 0; }
+// Lengths are under 2^31 and a chunk under 2^24 rows: tokens count in 32 bits, positions (which may be
+// negative) in 64.
+__device__ __forceinline__ int64_t paged_kq(const PagedGeometry& g, int64_t n) {
+  return (int64_t)quotient((uint32_t)n, g.R, g.flush_magic) * g.R;
+}
+__device__ __forceinline__ int64_t paged_vq(const PagedGeometry& g, int64_t n) { return n > g.R ? n - g.R : 0; }
+// Window row of token t.
+__device__ __forceinline__ uint32_t ring_row(const PagedGeometry& g, int64_t t) {
+  return (uint32_t)t - quotient((uint32_t)t, 2 * g.R, g.ring_magic) * 2 * g.R;
+}
+// Token of its page.
+__device__ __forceinline__ uint32_t token_in_page(const PagedGeometry& g, int64_t t) {
+  return (uint32_t)t - quotient((uint32_t)(t / kPagedBlock), g.page_blocks, g.page_magic) * g.P;
+}
 
 // Word (of a lane's words) and bit of element j of fragment f.
 __host__ __device__ inline uint32_t paged_word(uint32_t bits, uint32_t f, uint32_t j) {

@@ -83,10 +83,11 @@ template <class T>
 __device__ __forceinline__ const T* row_of(const PagedGeometry& g, const void* window, const PagedSequence& s,
                                            uint32_t head, int64_t t, const PagedRows& rows) {
   if (t < s.n)
-    return static_cast<const T*>(window) + (((uint64_t)s.slot * g.heads + head) * 2 * g.R + (uint64_t)t % (2 * g.R)) * g.D;
+    return static_cast<const T*>(window) + (((uint64_t)s.slot * g.heads + head) * 2 * g.R + ring_row(g, t)) * g.D;
   return static_cast<const T*>(rows.p) + (uint64_t)(s.row0 + (t - s.n)) * rows.stride + (uint64_t)head * g.D;
 }
 
+// Elements d .. d + 7 of a row of D, zeros behind its end (d < D).
 template <class T>
 __device__ __forceinline__ typename Row<T>::Frag load_frag(const T* p, bool vec, uint32_t d, uint32_t D) {
   typename Row<T>::Frag f;
@@ -96,7 +97,10 @@ __device__ __forceinline__ typename Row<T>::Frag load_frag(const T* p, bool vec,
     if constexpr (sizeof(T) == 4) e[1] = reinterpret_cast<const uint4*>(p + d)[1];
   } else {
 #pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) f[j] = d + j < D ? p[d + j] : (T)0.f;
+    for (uint32_t j = 0; j < 8; ++j) {
+      const T x = p[d + j < D ? d + j : D - 1];
+      f[j] = d + j < D ? x : (T)0.f;
+    }
   }
   return f;
 }
@@ -108,9 +112,9 @@ __device__ float value_of(const PagedAttention& a, const PagedSequence& s, const
   const PagedGeometry& g = a.c.geo;
   if (t >= vq) return (float)row_of<T>(g, a.c.vwin, s, head, t, a.values)[d];
   if (rec == nullptr) return 0.f;
-  const uint32_t in_page = (uint32_t)((uint64_t)t % g.P), tau = in_page % 32, j = tau % 4 + tau / 16 * 4;
-  const uint32_t* words = rec + g.vcodes_at() + (uint64_t)(in_page / 32) * g.block_words() + (tau % 16 / 4 * 16 + d % 16) * g.lane_words();
-  const float2 pair = reinterpret_cast<const float2*>(rec + g.vparams_at())[(uint64_t)in_page * g.ncg() + d / g.G];
+  const uint32_t in_page = token_in_page(g, t), tau = in_page % 32, j = tau % 4 + tau / 16 * 4;
+  const uint32_t* words = rec + g.vcodes_at + (uint64_t)(in_page / 32) * g.block_words() + (tau % 16 / 4 * 16 + d % 16) * g.lane_words();
+  const float2 pair = reinterpret_cast<const float2*>(rec + g.vparams_at)[(uint64_t)in_page * g.ncg + quotient(d, g.G, g.group_magic)];
   return (float)(T)decoded<T>(words[paged_word(g.bits, d / 16, j)] >> paged_bit(g.bits, d / 16, j) & g.levels(), pair);
 }
 
@@ -126,7 +130,13 @@ struct RowsPlan {
 };
 // Whether the kernels of few rows take this cache (else the chunk kernel takes everything).
 bool paged_rows_take(const PagedGeometry& g);
-template <class T>
+// Column groups by registers: the codes of a turn's blocks are 16 or 32 words a lane, once for keys and once
+// for values.
+__host__ __device__ constexpr int rows_most_blocks(uint32_t bits, uint32_t S) {
+  return S * bits / 2 <= 8 ? 4 : S * bits / 2 <= 16 ? 2 : 1;
+}
+// HALVES: G is an odd multiple of 16 (a block's halves may lie in two groups).
+template <class T, bool HALVES>
 hipError_t launch_paged_rows(const PagedAttention& a, const RowsPlan& p, float* partial, hipStream_t stream);
 
 }  // namespace kivi

@@ -31,6 +31,7 @@
 namespace kivi {
 namespace {
 
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
@@ -152,10 +153,10 @@ __device__ __forceinline__ uint32_t block_at(const Walk& w, uint32_t place) {
 // blocks. In a split of packed blocks each of the four waves takes BLOCKS at a time. Per turn: the
 // keys' pairs and codes are there; the values' are fetched while the logits are computed, the next
 // turn's keys while the output is.
-template <class T, int BITS, int S, int BLOCKS>
+template <class T, int BITS, int S, int BLOCKS, bool HALVES>
 __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPlan plan, float* partial) {
   constexpr int DP = 32 * S, F = 2 * S, LW = S * BITS / 2, ROWS = 16 / BLOCKS, NT = sizeof(T) == 4 ? 3 : 2;
-  constexpr int kKeyLoads = (S + 3) / 4, kValueLoads = (S + 1) / 2;
+  constexpr int kKeyLoads = (S + 3) / 4, kValueLoads = HALVES ? (S + 1) / 2 : (S + 3) / 4;  // float4s of pairs per lane
   constexpr uint32_t kQueryPitch = DP + 4, kKeyPitch = key_pitch(S);
   extern __shared__ __align__(16) float lds[];
   const PagedGeometry& g = a.c.geo;
@@ -177,7 +178,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
   if (tail ? part.count == part.mains : turn > part.mains) return;
   const uint32_t split = tail ? part.mains : turn - 1;
 
-  const uint32_t D = g.D, G = g.G, ncg = g.ncg(), per = G / 16;
+  const uint32_t D = g.D, G = g.G, ncg = g.ncg, per = G / 16;
   const uint32_t row = row0 + r < rows ? row0 + r : rows - 1;
   const int64_t pos = w.total - s.m + row / gq;
   const int64_t left = a.window != 0 ? pos - (int64_t)a.window : -1;
@@ -237,94 +238,103 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
     const int64_t first_pos = w.total - s.m + row0 / gq, last_left = a.window != 0 ? w.hi - 1 - (int64_t)a.window : -1;
     const uint32_t all_to = first_pos < 0 ? 0 : (uint32_t)((first_pos + 1) / kPagedBlock);
     const uint32_t all_from = last_left < 0 ? 0 : (uint32_t)((last_left + kPagedBlock) / kPagedBlock);
-    // where the words of this lane's float4s of pairs go
-    uint32_t kput[kKeyLoads], vput[kValueLoads];
+    // this lane's float4s of a block's pairs, and where their words go in LDS; lanes past the end take the last
+    uint32_t kget[kKeyLoads], kput[kKeyLoads], vget[kValueLoads], vput[kValueLoads];
 #pragma unroll
     for (int i = 0; i < kKeyLoads; ++i) {
-      const uint32_t at = 4 * (lane + 64 * i);
-      kput[i] = at / (16 * S) * kKeyPitch + at % (16 * S);
+      kget[i] = lane + 64 * i < 16 * S ? lane + 64 * i : 16 * S - 1;
+      kput[i] = 4 * kget[i] / (16 * S) * kKeyPitch + 4 * kget[i] % (16 * S);
     }
 #pragma unroll
     for (int i = 0; i < kValueLoads; ++i) {
-      const uint32_t at = 4 * (lane + 64 * i);
-      vput[i] = at / (8 * ncg) * vpitch + at % (8 * ncg);
+      vget[i] = lane + 64 * i < 16 * ncg ? lane + 64 * i : 16 * ncg - 1;
+      vput[i] = 4 * vget[i] / (8 * ncg) * vpitch + 4 * vget[i] % (8 * ncg);
     }
-    // blocks of a turn: number, place in the page, record (null: past the end, or no page)
+    // Blocks of a turn: number, place in the page, record. One past the end or of no page is read from the
+    // pool's first page (some codes and pairs) and seen by no row. Lane b looks up block b a turn ahead.
     uint32_t block[BLOCKS], inner[BLOCKS];
     const uint32_t* rec[BLOCKS];
-    const auto locate = [&](uint32_t at) {
+    bool held[BLOCKS];
+    uint32_t look_block, look_inner;
+    int32_t look_page;
+    const auto look_up = [&](uint32_t at) {
+      const uint32_t place = at + lane % BLOCKS;
+      look_block = block_at(w, place < to ? place : to - 1);
+      const uint32_t page = quotient(look_block, g.page_blocks, g.page_magic);
+      look_inner = look_block - page * g.page_blocks;
+      look_page = page < a.b.per_sequence && place < to ? s.table[page] : -1;
+    };
+    const auto locate = [&] {
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) {
-        block[b] = block_at(w, at + b);
-        rec[b] = nullptr;
-        if (at + b >= to) continue;
-        const uint32_t page = quotient(block[b], g.page_blocks, g.page_magic);
-        inner[b] = block[b] - page * g.page_blocks;
-        rec[b] = paged_record_of(a.c, a.b, s, head, page);
+        block[b] = __builtin_amdgcn_readlane(look_block, b);
+        inner[b] = __builtin_amdgcn_readlane(look_inner, b);
+        const uint32_t page = __builtin_amdgcn_readlane(look_page, b);
+        held[b] = page < g.pages;
+        rec[b] = a.c.pages + ((uint64_t)(held[b] ? page : 0) * g.heads + head) * g.record_words;
       }
     };
     uint32_t kc[BLOCKS][LW], vc[BLOCKS][LW];
-    float4 kp[BLOCKS][kKeyLoads], vp[BLOCKS][kValueLoads];
+    f32x4 kp[BLOCKS][kKeyLoads], vp[BLOCKS][kValueLoads];
     const auto load_words = [&](uint32_t(&words)[LW], const uint32_t* from) {
       if constexpr (LW % 4 == 0) {
 #pragma unroll
-        for (int i = 0; i < LW / 4; ++i) *reinterpret_cast<uint4*>(words + 4 * i) = reinterpret_cast<const uint4*>(from)[i];
+        for (int i = 0; i < LW / 4; ++i) {
+          const uint4 x = reinterpret_cast<const uint4*>(from)[i];
+          words[4 * i] = x.x, words[4 * i + 1] = x.y, words[4 * i + 2] = x.z, words[4 * i + 3] = x.w;
+        }
       } else if constexpr (LW % 2 == 0) {
 #pragma unroll
-        for (int i = 0; i < LW / 2; ++i) *reinterpret_cast<uint2*>(words + 2 * i) = reinterpret_cast<const uint2*>(from)[i];
+        for (int i = 0; i < LW / 2; ++i) {
+          const uint2 x = reinterpret_cast<const uint2*>(from)[i];
+          words[2 * i] = x.x, words[2 * i + 1] = x.y;
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < LW; ++i) words[i] = from[i];
       }
     };
-    const auto load_key_pairs = [&](float4(&pairs)[kKeyLoads], const uint32_t* record, uint32_t in_page) {
-      const float4* from = reinterpret_cast<const float4*>(record + g.kparams_at() + quotient(in_page, G, g.group_magic) * (DP * 2));
+    const auto load_key_pairs = [&](f32x4(&pairs)[kKeyLoads], const uint32_t* record, uint32_t in_page) {
+      const f32x4* from = reinterpret_cast<const f32x4*>(record + g.kparams_at + quotient(in_page, G, g.group_magic) * (DP * 2));
 #pragma unroll
-      for (int i = 0; i < kKeyLoads; ++i)
-        if (16 * S % 64 == 0 || lane + 64 * i < 16 * S) pairs[i] = from[lane + 64 * i];
+      for (int i = 0; i < kKeyLoads; ++i) pairs[i] = from[kget[i]];
     };
     const auto load_keys = [&] {
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) {
-        if (rec[b] == nullptr) continue;
         load_key_pairs(kp[b], rec[b], inner[b] * kPagedBlock);
         load_words(kc[b], rec[b] + inner[b] * (DP * BITS) + lane * LW);
       }
     };
-    const auto put_key_pairs = [&](int b, const float4(&from)[kKeyLoads]) {
+    const auto put_key_pairs = [&](int b, const f32x4(&from)[kKeyLoads]) {
 #pragma unroll
-      for (int i = 0; i < kKeyLoads; ++i)
-        if (16 * S % 64 == 0 || lane + 64 * i < 16 * S) *reinterpret_cast<float4*>(kpairs + b * 4 * kKeyPitch + kput[i]) = from[i];
+      for (int i = 0; i < kKeyLoads; ++i) *reinterpret_cast<f32x4*>(kpairs + b * 4 * kKeyPitch + kput[i]) = from[i];
     };
 
     uint32_t at = split * part.per + wave * BLOCKS;
     if (at < to) {
-      locate(at);
+      look_up(at);
+      locate();
       load_keys();
+      look_up(at + 4 * BLOCKS);
     }
     while (at < to) {
-      bool inside = true, was[BLOCKS];  // every block is there and seen by every row
+      bool inside = true;  // every row sees every token of the turn
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) {
-        was[b] = rec[b] != nullptr;
-        inside &= was[b] && block[b] >= all_from && block[b] < all_to;
-      }
-
+      for (int b = 0; b < BLOCKS; ++b) inside &= held[b] && block[b] >= all_from && block[b] < all_to;
       // ---- logits of eight tokens per lane: 16 half + 4 q + i
       wave_fence();
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b)
-        if (was[b]) put_key_pairs(b, kp[b]);
+      for (int b = 0; b < BLOCKS; ++b) put_key_pairs(b, kp[b]);
       wave_fence();
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) {
-        if (!was[b]) continue;
-        const float4* from = reinterpret_cast<const float4*>(rec[b] + g.vparams_at() + inner[b] * (kPagedBlock * 2) * ncg);
+        const f32x4* from = reinterpret_cast<const f32x4*>(rec[b] + g.vparams_at + inner[b] * (kPagedBlock * 2) * ncg);
 #pragma unroll
-        for (int i = 0; i < kValueLoads; ++i)
-          if (lane + 64 * i < 16 * ncg) vp[b][i] = from[lane + 64 * i];
-        load_words(vc[b], rec[b] + g.vcodes_at() + inner[b] * (DP * BITS) + lane * LW);
+        for (int i = 0; i < kValueLoads; ++i) vp[b][i] = from[vget[i]];
+        load_words(vc[b], rec[b] + g.vcodes_at + inner[b] * (DP * BITS) + lane * LW);
       }
+      __builtin_amdgcn_sched_barrier(0);  // phases one after the other: interleaved, they want more registers than there are
       float x[8];
       uint32_t unseen = 0;  // bit j: this lane's row does not see its token j
       {
@@ -337,28 +347,29 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
           for (int i = 0; i < S; ++i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              const float4 sz = *reinterpret_cast<const float4*>(pairs + 16 * i + 4 * j);
-              const float2 qq = *reinterpret_cast<const float2*>(qrow + 8 * i + 2 * j);
+              const f32x4 sz = *reinterpret_cast<const f32x4*>(pairs + 16 * i + 4 * j);
+              const f32x2 qq = *reinterpret_cast<const f32x2*>(qrow + 8 * i + 2 * j);
               uint32_t t[NT];
               terms_of<NT>(qq.x * sz.x, qq.y * sz.z, t);
 #pragma unroll
               for (int k = 0; k < NT; ++k) qk[i][k][j] = t[k];
               qz = fmaf(qq.x, sz.y, fmaf(qq.y, sz.w, qz));
             }
+            __builtin_amdgcn_sched_barrier(0);
           }
           qz += __shfl_xor(qz, 16);
           qz += __shfl_xor(qz, 32);
         };
         fold();
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          if (half == 1 && G % 32 != 0) {
+          if (HALVES && half == 1) {
             // the second 16 tokens of a block may lie in the next group
             wave_fence();
 #pragma unroll
             for (int b = 0; b < BLOCKS; ++b) {
-              if (!was[b]) continue;
-              float4 more[kKeyLoads];
+              f32x4 more[kKeyLoads];
               load_key_pairs(more, rec[b], inner[b] * kPagedBlock + 16);
               put_key_pairs(b, more);
             }
@@ -368,7 +379,6 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
           f32x4 mine = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int b = 0; b < BLOCKS; ++b) {
-            if (!was[b]) continue;
             f32x4 c = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int i = 0; i < S; ++i) {
@@ -383,6 +393,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) mine[i] = group == b ? c[i] : mine[i];
+            __builtin_amdgcn_sched_barrier(0);
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[4 * half + i] = (mine[i] + qz) * scale;
@@ -395,72 +406,75 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b) {
           t0 = group == b ? (int64_t)block[b] * kPagedBlock : t0;
-          there = group == b ? was[b] : there;
+          there = group == b ? held[b] : there;
         }
         const int see_to = there ? clamped(pos - t0, -1, 31) : -1, see_from = clamped(left - t0, -1, 31);
         const int sinks = clamped((int64_t)a.sinks - t0, 0, 32);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int tau = j / 4 * 16 + 4 * (int)q + j % 4;
-          if (tau <= see_to && (tau > see_from || tau < sinks)) continue;
-          x[j] = -INFINITY;
-          unseen |= 1u << j;
+          const bool seen = tau <= see_to && (tau > see_from || tau < sinks);
+          x[j] = seen ? x[j] : -INFINITY;
+          unseen |= seen ? 0u : 1u << j;
         }
       }
       weigh(x);
 
       // ---- output: the values' pairs go to LDS, the next turn's keys are fetched
 #pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) {
-        if (!was[b]) continue;
+      for (int b = 0; b < BLOCKS; ++b)
 #pragma unroll
-        for (int i = 0; i < kValueLoads; ++i)
-          if (lane + 64 * i < 16 * ncg) *reinterpret_cast<float4*>(vpairs + b * vblock + vput[i]) = vp[b][i];
-      }
+        for (int i = 0; i < kValueLoads; ++i) *reinterpret_cast<f32x4*>(vpairs + b * vblock + vput[i]) = vp[b][i];
       wave_fence();
       at += 4 * BLOCKS;
       if (at < to) {
-        locate(at);
+        locate();
         load_keys();
+        look_up(at + 4 * BLOCKS);
       }
-      uint32_t pk[BLOCKS][NT][4];  // (p s) of block b in the columns of group b, else zero
+      __builtin_amdgcn_sched_barrier(0);
+      constexpr int kStep = HALVES ? 1 : 2;  // fragments that lie in one group of channels whatever G is
       const float* pairs = vpairs + group * vblock + q * vpitch;
 #pragma unroll
-      for (int f = 0; f < F; ++f) {
-        if (f % per == 0) {
-          const uint32_t cg = f / per;
-          float y[8], z = 0.f;
+      for (int f0 = 0; f0 < F; f0 += kStep) {
+        const uint32_t cg = quotient(f0, per, g.fragment_magic);
+        float y[8], z = 0.f;
+        f32x2 sz[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            float2 sz = *reinterpret_cast<const float2*>(pairs + j / 4 * 4 * vpitch + (j % 4 * ncg + cg) * 2);
-            // what is not seen has no weight, whatever its pair
-            if (!inside && (unseen >> j & 1)) sz = make_float2(0.f, 0.f);
-            y[j] = x[j] * sz.x;
-            z = fmaf(x[j], sz.y, z);
-          }
-          zacc[f] += z;
+        for (int j = 0; j < 8; ++j) sz[j] = *reinterpret_cast<const f32x2*>(pairs + j / 4 * 4 * vpitch + (j % 4 * ncg + cg) * 2);
+        if (!inside) {
+          // what is not seen has no weight, whatever its pair
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t t[NT];
-            terms_of<NT>(y[2 * j], y[2 * j + 1], t);
+          for (int j = 0; j < 8; ++j) sz[j] = unseen >> j & 1 ? f32x2{0.f, 0.f} : sz[j];
+        }
 #pragma unroll
-            for (int b = 0; b < BLOCKS; ++b)
+        for (int j = 0; j < 8; ++j) {
+          y[j] = x[j] * sz[j].x;
+          z = fmaf(x[j], sz[j].y, z);
+        }
+        zacc[f0] += cg * per == (uint32_t)f0 ? z : 0.f;
+        uint32_t pk[BLOCKS][NT][4];  // (p s) of block b in the columns of group b, else zero
 #pragma unroll
-              for (int k = 0; k < NT; ++k) pk[b][k][j] = BLOCKS == 1 || group == b ? t[k] : 0u;
-          }
+        for (int j = 0; j < 4; ++j) {
+          uint32_t t[NT];
+          terms_of<NT>(y[2 * j], y[2 * j + 1], t);
+#pragma unroll
+          for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+            for (int k = 0; k < NT; ++k) pk[b][k][j] = BLOCKS == 1 || group == b ? t[k] : 0u;
         }
 #pragma unroll
         for (int b = 0; b < BLOCKS; ++b) {
-          if (!was[b]) continue;
-          const bf16x8 codes = codes_of<BITS>(vc[b], f);
 #pragma unroll
           for (int k = 0; k < NT; ++k) {
             Operand o;
 #pragma unroll
             for (int j = 0; j < 4; ++j) o.u[j] = pk[b][k][j];
-            acc[f] = mul16(codes, o.v, acc[f]);
+#pragma unroll
+            for (int f = f0; f < f0 + kStep; ++f) acc[f] = mul16(codes_of<BITS>(vc[b], f), o.v, acc[f]);
           }
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
   } else {
@@ -479,6 +493,26 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
       const int see_to = group == 0 ? clamped(pos - t0, -1, 31) : -1, see_from = clamped(left - t0, -1, 31);
       const int sinks = clamped((int64_t)a.sinks - t0, 0, 32), held = rec != nullptr ? 0 : kend;
       const auto seen = [&](int tau) { return tau <= see_to && (tau > see_from || tau < sinks) && tau >= held; };
+      // values that lie as rows, eight lanes a token, 64 channels at a time: fetched while the logits are
+      // computed where the registers hold them
+      constexpr int kChunks = (F + 3) / 4;
+      constexpr bool kAhead = kChunks * sizeof(T) <= 8;
+      Frag values[kAhead ? kChunks : 1][4];
+      const auto load_values = [&](int chunk, Frag(&to)[4]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int tau = 8 * k + (int)(lane / 8);
+          const uint32_t d = 64 * chunk + lane % 8 * 8;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) to[k][j] = (T)0.f;
+          if (tau >= vend && tau < end && d < D)
+            to[k] = load_frag(row_of<T>(g, a.c.vwin, s, head, t0 + tau, a.values), t0 + tau < s.n ? wvec : a.values.vec != 0, d, D);
+        }
+      };
+      if constexpr (kAhead) {
+#pragma unroll
+        for (int i = 0; i < kChunks; ++i) load_values(i, values[i]);
+      }
       float x[8];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
@@ -487,14 +521,14 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
         const T* p = !packed && tau < end ? row_of<T>(g, a.c.kwin, s, head, t0 + tau, a.keys) : nullptr;
         const bool vec = t0 + tau < s.n ? wvec : a.keys.vec != 0;
         const uint32_t* words = rec + inner * (DP * BITS) + lane * LW;
-        const float2* pairs = reinterpret_cast<const float2*>(rec + g.kparams_at()) +
+        const float2* pairs = reinterpret_cast<const float2*>(rec + g.kparams_at) +
                               quotient(inner * kPagedBlock + tau, G, g.group_magic) * DP + 8 * S * q;
         Frag k8[S];
 #pragma unroll
         for (int k = 0; k < S; ++k) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) k8[k][j] = (T)0.f;
-          if (p != nullptr) {
+          if (p != nullptr && 8 * S * q + 8 * k < D) {
             k8[k] = load_frag(p, vec, 8 * S * q + 8 * k, D);
           } else if (packed && rec != nullptr) {
 #pragma unroll
@@ -513,6 +547,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[4 * half + k] = seen(16 * half + 4 * (int)q + k) ? c[k] * scale : -INFINITY;
+        __builtin_amdgcn_sched_barrier(0);
       }
       weigh(x);
       Frag p8;
@@ -521,18 +556,15 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
       uint32_t bad = 0;  // tokens with a value that is not finite: it goes to the rows that see them alone
 #pragma unroll
       for (int f0 = 0; f0 < F; f0 += 4) {
+        if constexpr (!kAhead) load_values(f0 / 4, values[0]);
         wave_fence();
         // 32 tokens of 64 channels: eight lanes a token
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int tau = 8 * k + (int)(lane / 8);
-          const uint32_t to = lane % 8 * 8, d = 16 * f0 + to;
+          const uint32_t to = lane % 8 * 8;
           if (tau < vend) continue;
-          Frag v8;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v8[j] = (T)0.f;
-          if (d < D && tau < end)
-            v8 = load_frag(row_of<T>(g, a.c.vwin, s, head, t0 + tau, a.values), t0 + tau < s.n ? wvec : a.values.vec != 0, d, D);
+          Frag v8 = values[kAhead ? f0 / 4 : 0][k];
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             if (!(fabsf((float)v8[j]) <= kLargest)) {
@@ -549,18 +581,28 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
           }
         }
         if (vend > 0) {
-          const int64_t t_end = t0 + vend;
-#pragma unroll 1
-          for (int k = 0; k < 4 * 8; ++k) {  // one token and channel per lane
-            const int j = k % 8, tau = j / 4 * 16 + 4 * (int)q + j % 4;
-            const uint32_t to = k / 8 * 16 + col, d = 16 * f0 + to;
-            if (t0 + tau >= t_end) continue;
-            float v = d < D ? value_of<T>(a, s, rec, head, t0 + tau, vq, d) : 0.f;
-            if (!(fabsf(v) <= kLargest)) {
-              bad |= 1u << tau;
-              v = 0.f;
+          // packed ones among them: eight tokens of one channel a lane
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            if (f0 + k >= F) continue;
+            const uint32_t d = 16 * (f0 + k) + col;
+            const uint32_t* from = rec != nullptr ? rec : a.c.pages;
+            const uint32_t* words = from + g.vcodes_at + inner * (DP * BITS) + lane * LW;
+            const float2* pairs = reinterpret_cast<const float2*>(from + g.vparams_at) + inner * kPagedBlock * ncg +
+                                  quotient(d < D ? d : D - 1, G, g.group_magic);
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              v[j] = decoded<T>(words[paged_word(BITS, f0 + k, j)] >> paged_bit(BITS, f0 + k, j) & ((1u << BITS) - 1),
+                                pairs[(j / 4 * 16 + 4 * q + j % 4) * ncg]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const int tau = j / 4 * 16 + 4 * (int)q + j % 4;
+              const bool fine = fabsf(v[j]) <= kLargest, real = d < D && rec != nullptr;
+              if (tau >= vend) continue;
+              bad |= real && !fine ? 1u << tau : 0u;
+              tile[tau * kTilePitch + 16 * k + col] = (T)(real && fine ? v[j] : 0.f);
             }
-            tile[tau * kTilePitch + to] = (T)v;
           }
         }
         wave_fence();
@@ -572,6 +614,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
           for (int j = 0; j < 8; ++j) v8[j] = tile[(j / 4 * 16 + 4 * q + j % 4) * kTilePitch + 16 * k + col];
           acc[f0 + k] = mul16(v8, p8, acc[f0 + k]);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
       if (__any(bad != 0)) {
 #pragma unroll
@@ -703,11 +746,11 @@ __global__ void __launch_bounds__(256) k_paged_rows_join(PagedAttention a, RowsP
     out[d] = (T)((part_out[0][d] + part_out[1][d] + part_out[2][d] + part_out[3][d]) * inv);
 }
 
-template <class T, int BITS, int S, int BLOCKS>
+template <class T, int BITS, int S, int BLOCKS, bool HALVES>
 hipError_t rows_launch(const PagedAttention& a, const RowsPlan& p, float* partial, hipStream_t stream) {
   const PagedGeometry& g = a.c.geo;
-  const size_t bytes = rows_lds_words<T>(S, g.ncg(), BLOCKS) * 4;
-  auto kernel = k_paged_rows<T, BITS, S, BLOCKS>;
+  const size_t bytes = rows_lds_words<T>(S, g.ncg, BLOCKS) * 4;
+  auto kernel = k_paged_rows<T, BITS, S, BLOCKS, HALVES>;
   hipError_t e = raise_lds_limit(reinterpret_cast<const void*>(kernel), bytes);
   if (e != hipSuccess) return e;
   constexpr uint32_t kTile = 16 / BLOCKS;
@@ -717,34 +760,37 @@ hipError_t rows_launch(const PagedAttention& a, const RowsPlan& p, float* partia
   return hipGetLastError();
 }
 
-template <class T, int BITS, int S>
+template <class T, int BITS, int S, bool HALVES>
 hipError_t rows_blocks(const PagedAttention& a, const RowsPlan& p, float* partial, hipStream_t stream) {
-  switch (p.blocks) {
-    case 4: return rows_launch<T, BITS, S, 4>(a, p, partial, stream);
-    case 2: return rows_launch<T, BITS, S, 2>(a, p, partial, stream);
-    default: return rows_launch<T, BITS, S, 1>(a, p, partial, stream);
+  constexpr int kMost = rows_most_blocks(BITS, S);
+  if constexpr (kMost >= 4) {
+    if (p.blocks == 4) return rows_launch<T, BITS, S, 4, HALVES>(a, p, partial, stream);
   }
+  if constexpr (kMost >= 2) {
+    if (p.blocks == 2) return rows_launch<T, BITS, S, 2, HALVES>(a, p, partial, stream);
+  }
+  return p.blocks == 1 ? rows_launch<T, BITS, S, 1, HALVES>(a, p, partial, stream) : hipErrorInvalidValue;
 }
 
-template <class T, int BITS>
+template <class T, int BITS, bool HALVES>
 hipError_t rows_dims(const PagedAttention& a, const RowsPlan& p, float* partial, hipStream_t stream) {
   switch (a.c.geo.S()) {
-    case 2: return rows_blocks<T, BITS, 2>(a, p, partial, stream);
-    case 3: return rows_blocks<T, BITS, 3>(a, p, partial, stream);
-    case 4: return rows_blocks<T, BITS, 4>(a, p, partial, stream);
-    case 8: return rows_blocks<T, BITS, 8>(a, p, partial, stream);
+    case 2: return rows_blocks<T, BITS, 2, HALVES>(a, p, partial, stream);
+    case 3: return rows_blocks<T, BITS, 3, HALVES>(a, p, partial, stream);
+    case 4: return rows_blocks<T, BITS, 4, HALVES>(a, p, partial, stream);
+    case 8: return rows_blocks<T, BITS, 8, HALVES>(a, p, partial, stream);
     default: return hipErrorInvalidValue;  // paged_rows_take
   }
 }
 
 }  // namespace
 
-template <class T>
+template <class T, bool HALVES>
 hipError_t launch_paged_rows(const PagedAttention& a, const RowsPlan& p, float* partial, hipStream_t stream) {
   switch (a.c.geo.bits) {
-    case 2: return rows_dims<T, 2>(a, p, partial, stream);
-    case 4: return rows_dims<T, 4>(a, p, partial, stream);
-    default: return rows_dims<T, 8>(a, p, partial, stream);
+    case 2: return rows_dims<T, 2, HALVES>(a, p, partial, stream);
+    case 4: return rows_dims<T, 4, HALVES>(a, p, partial, stream);
+    default: return rows_dims<T, 8, HALVES>(a, p, partial, stream);
   }
 }
 
