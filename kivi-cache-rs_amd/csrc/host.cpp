@@ -1627,14 +1627,16 @@ Status create_paged(const kivi_config* config, size_t heads, size_t head_dim, in
   g.finish();
   KIVI_TRY(mul4(num_pages, heads, g.record_words, 4, &pages_bytes));
   KIVI_TRY(mul4(num_slots, heads, 2 * config->residual_length, 1, &rows));
-  KIVI_TRY(mul4(rows, head_dim, g.type_bytes(), 1, &window_bytes));
+  KIVI_TRY(mul4(rows, g.DW, g.type_bytes(), 1, &window_bytes));
   c->cfg = *config;
   KIVI_TRY(current_device(&c->device));
   KIVI_TRY(c->pages.alloc(pages_bytes, nullptr, "paged cache"));
   KIVI_TRY(c->kwin.alloc(window_bytes, nullptr, "paged cache windows"));
   KIVI_TRY(c->vwin.alloc(window_bytes, nullptr, "paged cache windows"));
-  // the channels behind head_dim are never written and have to be zero
+  // what lies behind head_dim is never written and has to be zero
   HIP_TRY(launch_fill_zero(c->pages.as<float>(), pages_bytes / 4, nullptr), "paged cache");
+  HIP_TRY(launch_fill_zero(c->kwin.as<float>(), window_bytes / 4, nullptr), "paged cache windows");
+  HIP_TRY(launch_fill_zero(c->vwin.as<float>(), window_bytes / 4, nullptr), "paged cache windows");
   return sync(nullptr, "paged cache");
 }
 
@@ -1683,7 +1685,8 @@ Status paged_rows(const kivi_paged& c, const PagedBatch& b, size_t heads, const 
   if (at % size != 0) return Err(KIVI_ERR_UNSUPPORTED, at % size, 0, "address % element size");
   out->p = p;
   out->stride = stride;
-  out->vec = at % 16 == 0 && stride * size % 16 == 0 && c.geo.D * size % 16 == 0;
+  out->pitch = c.geo.D;
+  out->vec = at % 16 == 0 && stride * size % 16 == 0 && c.geo.D % 8 == 0;
   return Status{};
 }
 
@@ -2363,7 +2366,7 @@ kivi_status kivi_paged_attention_device(const kivi_paged* cache, const kivi_page
         return Err(KIVI_ERR_UNSUPPORTED, reinterpret_cast<uintptr_t>(workspace) % 16, 0, "workspace % 16");
     }
     DeviceScope scope(cache->device);
-    HIP_TRY(launch_paged_attention(a, static_cast<float*>(workspace), static_cast<hipStream_t>(stream)), "paged attention");
+    HIP_TRY(launch_paged_attention(a, workspace, static_cast<hipStream_t>(stream)), "paged attention");
     return Status{};
   });
 }

@@ -66,10 +66,10 @@ __device__ __forceinline__ float decoded(uint32_t code, float2 pair) {
 // The row of token t of one head: in the window while t < n, else new row t - n of the tensor.
 template <class T>
 __device__ __forceinline__ const T* token_row(const PagedGeometry& g, const T* window, const PagedSequence& s,
-                                              uint32_t head, int64_t t, const T* rows, uint64_t stride) {
+                                              uint32_t head, int64_t t, const T* rows, uint64_t stride, uint32_t pitch) {
   if (t < s.n)
-    return window + (((uint64_t)s.slot * g.heads + head) * 2 * g.R + ring_row(g, t)) * g.D;
-  return rows + (uint64_t)(s.row0 + (t - s.n)) * stride + (uint64_t)head * g.D;
+    return window + (((uint64_t)s.slot * g.heads + head) * 2 * g.R + ring_row(g, t)) * g.DW;
+  return rows + (uint64_t)(s.row0 + (t - s.n)) * stride + (uint64_t)head * pitch;
 }
 
 // (scale, zero) of the group of `count` elements at p, `stride` apart, by kReduce neighbouring lanes,
@@ -119,7 +119,6 @@ __global__ void __launch_bounds__(kThreads)
   const int64_t n = s.n, n2 = s.n + s.m;
   const uint32_t D = g.D, S = g.S(), LW = g.lane_words(), levels = g.levels();
   const float flevels = (float)levels;
-  const bool wvec = D * sizeof(T) % 16 == 0;
   const T* kw = static_cast<const T*>(c.kwin);
   const T* vw = static_cast<const T*>(c.vwin);
   const T* kr = static_cast<const T*>(keys.p);
@@ -140,8 +139,8 @@ __global__ void __launch_bounds__(kThreads)
       const int64_t t = lo + i / S;
       const uint32_t o = i % S * 8, d = ch0 + o;
       float x[8];
-      const T* row = token_row(g, kw, s, head, t, kr, keys.stride);
-      load8(row + d, t < n ? wvec : keys.vec != 0, d < D ? D - d : 0, x);
+      const T* row = token_row(g, kw, s, head, t, kr, keys.stride, keys.pitch);
+      load8(row + d, t < n || keys.vec != 0, d < D ? D - d : 0, x);
 #pragma unroll
       for (uint32_t j = 0; j < 8; ++j) tile[(uint32_t)(t - base) * pitch + o + j] = x[j];
     }
@@ -192,8 +191,8 @@ __global__ void __launch_bounds__(kThreads)
       const int64_t t = lo + i / oct;
       const uint32_t d = i % oct * 8;
       float x[8];
-      const T* row = token_row(g, vw, s, head, t, vr, values.stride);
-      load8(row + d, t < n ? wvec : values.vec != 0, d < D ? D - d : 0, x);
+      const T* row = token_row(g, vw, s, head, t, vr, values.stride, values.pitch);
+      load8(row + d, t < n || values.vec != 0, d < D ? D - d : 0, x);
 #pragma unroll
       for (uint32_t j = 0; j < 8; ++j) tile[(uint32_t)(t - base) * pitch + d + j] = x[j];
     }
@@ -235,10 +234,10 @@ __global__ void __launch_bounds__(kThreads)
   for (int64_t i = tid; lo + i / D < hi; i += kThreads) {
     const int64_t t = lo + i / D;
     const uint32_t d = (uint32_t)(i % D);
-    const uint64_t to = (((uint64_t)s.slot * g.heads + head) * 2 * g.R + ring_row(g, t)) * D + d;
+    const uint64_t to = (((uint64_t)s.slot * g.heads + head) * 2 * g.R + ring_row(g, t)) * g.DW + d;
     const uint64_t row = (uint64_t)(s.row0 + (t - n));
-    static_cast<T*>(c.kwin)[to] = kr[row * keys.stride + (uint64_t)head * D + d];
-    static_cast<T*>(c.vwin)[to] = vr[row * values.stride + (uint64_t)head * D + d];
+    static_cast<T*>(c.kwin)[to] = kr[row * keys.stride + (uint64_t)head * keys.pitch + d];
+    static_cast<T*>(c.vwin)[to] = vr[row * values.stride + (uint64_t)head * values.pitch + d];
   }
 }
 
@@ -256,7 +255,6 @@ __global__ void __launch_bounds__(kThreads)
   const int32_t from = first != nullptr ? first[blockIdx.z] : 0;
   const int64_t f0 = from > 0 ? from : 0, end = f0 + s.m, n = s.n;
   const uint32_t D = g.D, S = g.S(), LW = g.lane_words(), levels = g.levels(), oct = (D + 7) / 8, ncg = g.ncg;
-  const bool wvec = D * sizeof(T) % 16 == 0;
   const T* kw = static_cast<const T*>(c.kwin);
   const T* vw = static_cast<const T*>(c.vwin);
   T* kout = static_cast<T*>(const_cast<void*>(keys.p));
@@ -302,19 +300,19 @@ __global__ void __launch_bounds__(kThreads)
             x[j] = decoded(words[paged_word(g.bits, f, j)] >> paged_bit(g.bits, f, j) & levels, pairs[j]);
         }
       } else if (t < n) {
-        load8(token_row<T>(g, kw, s, head, t, nullptr, 0) + d, wvec, have, x);
+        load8(token_row<T>(g, kw, s, head, t, nullptr, 0, 0) + d, true, have, x);
       }
-      store8(kout + row * keys.stride + (uint64_t)head * D + d, keys.vec != 0, have, x);
+      store8(kout + row * keys.stride + (uint64_t)head * keys.pitch + d, keys.vec != 0, have, x);
       if (t < vq) {
 #pragma unroll
         for (uint32_t j = 0; j < 8; ++j) x[j] = rec != nullptr && j < have ? to_f(turned[tau * pitch + d + j]) : 0.f;
       } else if (t < n) {
-        load8(token_row<T>(g, vw, s, head, t, nullptr, 0) + d, wvec, have, x);
+        load8(token_row<T>(g, vw, s, head, t, nullptr, 0, 0) + d, true, have, x);
       } else {
 #pragma unroll
         for (uint32_t j = 0; j < 8; ++j) x[j] = 0.f;
       }
-      store8(vout + row * values.stride + (uint64_t)head * D + d, values.vec != 0, have, x);
+      store8(vout + row * values.stride + (uint64_t)head * values.pitch + d, values.vec != 0, have, x);
     }
     __syncthreads();
   }

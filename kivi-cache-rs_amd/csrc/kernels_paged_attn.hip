@@ -84,7 +84,6 @@ __global__ void __launch_bounds__(WAVES * 64)
   if (split >= part.count) return;
 
   const uint32_t D = g.D, S = g.S(), LW = g.lane_words(), levels = g.levels();
-  const bool wvec = D * sizeof(T) % 16 == 0;
   const int64_t kq = paged_kq(g, s.n), vq = paged_vq(g, s.n);
   const uint32_t row = tile_row + wave * 32 + col;
   const bool live = row < rows;
@@ -101,13 +100,11 @@ __global__ void __launch_bounds__(WAVES * 64)
 
   Frag q[DP / 16];
   {
-    const T* p = static_cast<const T*>(a.query.p) + (uint64_t)(s.row0 + token) * a.query.stride + (uint64_t)qhead * D;
+    const T* p = static_cast<const T*>(a.query.p) + (uint64_t)(s.row0 + token) * a.query.stride + (uint64_t)qhead * a.query.pitch;
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
       const uint32_t d = 16 * i + 8 * half;
-#pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) q[i][j] = (T)0.f;
-      if (d < D) q[i] = load_frag(p, a.query.vec != 0, d, D);
+      q[i] = d < g.DW ? load_frag(p, d) : zero_frag<T>();
     }
   }
   const float scale = a.scale * kLog2e;
@@ -148,8 +145,8 @@ __global__ void __launch_bounds__(WAVES * 64)
 #pragma unroll
           for (uint32_t j = 0; j < 8; ++j) f[j] = (T)0.f;
         }
-      } else if (t < w.hi && d < D) {
-        f = load_frag(row_of<T>(g, a.c.kwin, s, head, t, a.keys), t < s.n ? wvec : a.keys.vec != 0, d, D);
+      } else if (t < w.hi && d < g.DW) {
+        f = load_frag(row_of<T>(g, a.c.kwin, s, head, t, a.keys), d);
       } else {
 #pragma unroll
         for (uint32_t j = 0; j < 8; ++j) f[j] = (T)0.f;
@@ -322,6 +319,16 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// Rows as the kernels take them (whole 8-element pieces on 16 bytes), for a caller whose rows are not.
+template <class T>
+__global__ void __launch_bounds__(256) k_paged_align(PagedRows from, T* to, uint32_t D, uint32_t DW, uint32_t heads, uint64_t rows) {
+  const uint64_t all = rows * heads * DW;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (uint64_t)gridDim.x * 256) {
+    const uint32_t d = (uint32_t)(i % DW), h = (uint32_t)(i / DW % heads);
+    to[i] = d < D ? static_cast<const T*>(from.p)[i / DW / heads * from.stride + (uint64_t)h * from.pitch + d] : (T)0.f;
+  }
+}
+
 // How a call is cut. The lengths are device memory, so the plan goes by the host's bounds: sequences
 // shorter than those take fewer of the planned splits, and their other workgroups end at once.
 struct Plan {
@@ -362,8 +369,10 @@ Plan plan_of(const PagedGeometry& g, const PagedBatch& b, uint32_t qh, uint64_t 
       // blocks of a split and the splits of a walk over n tokens, at most `cap`
       const auto cut = [&](uint64_t n, uint64_t cap) {
         const uint64_t blocks = std::max<uint64_t>(1, (n + kPagedBlock - 1) / kPagedBlock);
-        const uint64_t least = std::max(blocks * heads * tiles / kRowsWorkgroups, (blocks + cap - 1) / cap);
-        r.least = (uint32_t)((std::max<uint64_t>(1, least) + turn - 1) / turn * turn);
+        // one to four turns a wave (what surrounds the turns costs about one), more where there are many
+        const uint64_t turns = std::clamp<uint64_t>(blocks * heads * tiles / turn / 1024, 1, 4);
+        const uint64_t least = std::max({turns * turn, blocks * heads * tiles / kRowsWorkgroups, (blocks + cap - 1) / cap});
+        r.least = (uint32_t)((least + turn - 1) / turn * turn);
         r.splits = (uint32_t)((blocks + r.least - 1) / r.least);
       };
       cut(all, kMostSplits);
@@ -408,12 +417,36 @@ hipError_t launch_chunk(const PagedAttention& a, const ChunkPlan& p, float* part
   return hipGetLastError();
 }
 
+// Bytes of the workspace in front of the partials, for rows that have to be aligned first.
+size_t aligned_bytes(const PagedGeometry& g, const PagedBatch& b, uint32_t qh) {
+  return ((size_t)b.rows * (qh + 2 * g.heads) * g.DW * g.type_bytes() + 255) / 256 * 256;
+}
+
 template <class T>
-hipError_t attention_typed(const PagedAttention& a, float* workspace, hipStream_t stream) {
+hipError_t align(PagedRows* r, T* to, const PagedAttention& a, uint32_t heads, hipStream_t stream) {
+  const PagedGeometry& g = a.c.geo;
+  const uint64_t all = (uint64_t)a.b.rows * heads * g.DW;
+  hipLaunchKernelGGL(k_paged_align<T>, dim3((uint32_t)std::min<uint64_t>((all + 255) / 256, 1u << 16)), dim3(256), 0, stream, *r, to,
+                     g.D, g.DW, heads, (uint64_t)a.b.rows);
+  *r = PagedRows{to, (uint64_t)heads * g.DW, g.DW, 1};
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t attention_typed(PagedAttention a, void* memory, hipStream_t stream) {
+  T* rows = static_cast<T*>(memory);
+  float* workspace = reinterpret_cast<float*>(static_cast<char*>(memory) + aligned_bytes(a.c.geo, a.b, a.qh));
+  hipError_t e = hipSuccess;
+  if (!a.query.vec) e = align(&a.query, rows, a, a.qh, stream);
+  rows += (uint64_t)a.b.rows * a.qh * a.c.geo.DW;
+  if (e == hipSuccess && a.keys.p != nullptr && !a.keys.vec) e = align(&a.keys, rows, a, a.c.geo.heads, stream);
+  rows += (uint64_t)a.b.rows * a.c.geo.heads * a.c.geo.DW;
+  if (e == hipSuccess && a.keys.p != nullptr && !a.values.vec) e = align(&a.values, rows, a, a.c.geo.heads, stream);
+  if (e != hipSuccess) return e;
   const Plan p = plan_of(a.c.geo, a.b, a.qh, a.window, a.sinks);
   for (uint32_t i = 0; i < p.row_launches; ++i) {
-    const hipError_t e = a.c.geo.G % 32 != 0 ? launch_paged_rows<T, true>(a, p.rows[i], workspace + p.rows_at[i], stream)
-                                             : launch_paged_rows<T, false>(a, p.rows[i], workspace + p.rows_at[i], stream);
+    e = a.c.geo.G % 32 != 0 ? launch_paged_rows<T, true>(a, p.rows[i], workspace + p.rows_at[i], stream)
+                            : launch_paged_rows<T, false>(a, p.rows[i], workspace + p.rows_at[i], stream);
     if (e != hipSuccess) return e;
   }
   if (!p.chunks) return hipSuccess;
@@ -434,10 +467,10 @@ bool paged_rows_take(const PagedGeometry& g) {
 }
 
 size_t paged_attention_workspace(const PagedGeometry& g, const PagedBatch& b, uint32_t qh) {
-  return plan_of(g, b, qh, 0, 0).floats * sizeof(float);
+  return aligned_bytes(g, b, qh) + plan_of(g, b, qh, 0, 0).floats * sizeof(float);
 }
 
-hipError_t launch_paged_attention(const PagedAttention& a, float* workspace, hipStream_t stream) {
+hipError_t launch_paged_attention(PagedAttention a, void* workspace, hipStream_t stream) {
   switch (a.c.geo.type) {
     case kPagedF32: return attention_typed<float>(a, workspace, stream);
     case kPagedF16: return attention_typed<_Float16>(a, workspace, stream);

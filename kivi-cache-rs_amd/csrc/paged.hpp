@@ -62,11 +62,13 @@ struct PagedGeometry {
   uint32_t type;   // PagedType
   // what follows from those (finish); offsets in words from a record
   uint32_t ncg, page_blocks;
+  uint32_t DW;     // D rounded up to 8: pitch of the windows' rows (zeros behind D)
   uint32_t kparams_at, vcodes_at, vparams_at, record_words;
   uint32_t page_magic, group_magic, fragment_magic, flush_magic, ring_magic;  // of P/32, G, max(1, G/16), R, 2R
 
   __host__ void finish() {
     ncg = D / G;
+    DW = (D + 7) / 8 * 8;
     page_blocks = P / kPagedBlock;
     kparams_at = page_blocks * block_words();
     vcodes_at = kparams_at + P / G * DP * 2;
@@ -88,7 +90,7 @@ struct PagedGeometry {
 struct PagedView {
   PagedGeometry geo;
   uint32_t* pages;
-  void* kwin;  // [slots][heads][2R][D]
+  void* kwin;  // [slots][heads][2R][DW]
   void* vwin;
 };
 
@@ -167,11 +169,12 @@ __host__ __device__ inline uint32_t paged_bit(uint32_t bits, uint32_t f, uint32_
   return bits == 2 ? 4 * j + 2 * (f & 1) : bits == 4 ? 8 * (j & 3) + 4 * (j >> 2) : 8 * (j & 3);
 }
 
-// Rows of a ragged tensor: row r, head h at p + r * stride + h * D (in elements). `vec`: every row
-// of a head starts on 16 bytes (32 for f32 would not be needed: it is read in halves).
+// Rows of a ragged tensor: row r, head h at p + r * stride + h * pitch (in elements). `vec`: every row of
+// a head is whole 8-element pieces on 16 bytes.
 struct PagedRows {
   const void* p;
   uint64_t stride;
+  uint32_t pitch;
   uint32_t vec;
 };
 
@@ -184,7 +187,7 @@ hipError_t launch_paged_read(const PagedView& c, const PagedBatch& b, const int3
 struct PagedAttention {
   PagedView c;
   PagedBatch b;
-  PagedRows query, keys, values;  // keys.p null: the new tokens are cached already
+  PagedRows query, keys, values;  // keys.p null: the new tokens are cached already. The kernels take `vec` ones.
   void* out;
   uint64_t out_stride;
   uint32_t out_vec;
@@ -193,6 +196,6 @@ struct PagedAttention {
   uint64_t window, sinks;  // window 0: none
 };
 size_t paged_attention_workspace(const PagedGeometry& g, const PagedBatch& b, uint32_t qh);
-hipError_t launch_paged_attention(const PagedAttention& a, float* workspace, hipStream_t stream);
+hipError_t launch_paged_attention(PagedAttention a, void* workspace, hipStream_t stream);
 
 }  // namespace kivi

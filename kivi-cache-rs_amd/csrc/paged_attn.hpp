@@ -14,6 +14,7 @@ constexpr float kLargest = 3.402823466e+38f;  // |x| <= kLargest: x is finite
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 // Eight elements of a row.
 template <class T>
@@ -83,26 +84,33 @@ template <class T>
 __device__ __forceinline__ const T* row_of(const PagedGeometry& g, const void* window, const PagedSequence& s,
                                            uint32_t head, int64_t t, const PagedRows& rows) {
   if (t < s.n)
-    return static_cast<const T*>(window) + (((uint64_t)s.slot * g.heads + head) * 2 * g.R + ring_row(g, t)) * g.D;
-  return static_cast<const T*>(rows.p) + (uint64_t)(s.row0 + (t - s.n)) * rows.stride + (uint64_t)head * g.D;
+    return static_cast<const T*>(window) + (((uint64_t)s.slot * g.heads + head) * 2 * g.R + ring_row(g, t)) * g.DW;
+  return static_cast<const T*>(rows.p) + (uint64_t)(s.row0 + (t - s.n)) * rows.stride + (uint64_t)head * rows.pitch;
 }
 
-// Elements d .. d + 7 of a row of D, zeros behind its end (d < D).
+// Elements d .. d + 7 of a row (d a multiple of 8 under DW).
 template <class T>
-__device__ __forceinline__ typename Row<T>::Frag load_frag(const T* p, bool vec, uint32_t d, uint32_t D) {
+__device__ __forceinline__ typename Row<T>::Frag load_frag(const T* p, uint32_t d) {
   typename Row<T>::Frag f;
-  if (vec && d + 8 <= D) {
-    uint4* e = reinterpret_cast<uint4*>(&f);
-    e[0] = reinterpret_cast<const uint4*>(p + d)[0];
-    if constexpr (sizeof(T) == 4) e[1] = reinterpret_cast<const uint4*>(p + d)[1];
-  } else {
-#pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
-      const T x = p[d + j < D ? d + j : D - 1];
-      f[j] = d + j < D ? x : (T)0.f;
-    }
-  }
+  u32x4* e = reinterpret_cast<u32x4*>(&f);
+  e[0] = reinterpret_cast<const u32x4*>(p + d)[0];
+  if constexpr (sizeof(T) == 4) e[1] = reinterpret_cast<const u32x4*>(p + d)[1];
   return f;
+}
+template <class T>
+__device__ __forceinline__ typename Row<T>::Frag zero_frag() {
+  typename Row<T>::Frag f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = (T)0.f;
+  return f;
+}
+// Whether any of the eight is infinite or NaN.
+template <class T>
+__device__ __forceinline__ bool wild(const typename Row<T>::Frag& f) {
+  bool any = false;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) any |= !(fabsf((float)f[j]) <= kLargest);
+  return any;
 }
 
 // Value (t, d) of one head, t among what the row tile walks; `rec` the record of t's page.

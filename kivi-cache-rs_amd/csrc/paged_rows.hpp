@@ -102,14 +102,13 @@ __host__ __device__ inline uint32_t rows_wave_words(uint32_t S, uint32_t ncg, ui
   const uint32_t k = 4 * key_pitch(S), v = value_block(ncg);
   return blocks * (k + v);
 }
-// Of the last blocks: values [32 tokens][64 channels], rows padded so that the four token quads of a
-// transposed read fall on different banks.
-constexpr uint32_t kTileChannels = 64;
+// Of the last blocks: values [32 tokens][DP], rows padded so that the four token quads of a transposed
+// read fall on different banks (16 bytes: four rows on are 16 words on).
 template <class T>
-__host__ __device__ constexpr uint32_t tile_pitch() { return kTileChannels + (sizeof(T) == 4 ? 4 : 4); }  // elements
+__host__ __device__ constexpr uint32_t tile_pitch(uint32_t S) { return 32 * S + 16 / sizeof(T); }  // elements
 template <class T>
 __host__ __device__ inline uint32_t wave_words(uint32_t S, uint32_t ncg, uint32_t blocks) {
-  const uint32_t pairs = rows_wave_words(S, ncg, blocks), tile = 32 * tile_pitch<T>() * sizeof(T) / 4;
+  const uint32_t pairs = rows_wave_words(S, ncg, blocks), tile = 32 * tile_pitch<T>(S) * sizeof(T) / 4;
   return ((pairs > tile ? pairs : tile) + 3) / 4 * 4;
 }
 // LDS of a workgroup of four waves: queries [rows][DP + 4], then the waves' pairs, whose place the
@@ -187,7 +186,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
   float* own = lds + ROWS * kQueryPitch + wave * wave_words<T>(S, ncg, BLOCKS);  // the wave's
   for (uint32_t i = tid; i < ROWS * DP; i += 256) {
     const uint32_t rr = i / DP, d = i % DP, ri = row0 + rr < rows ? row0 + rr : rows - 1;
-    const T* p = static_cast<const T*>(a.query.p) + (uint64_t)(s.row0 + ri / gq) * a.query.stride + (uint64_t)(head * gq + ri % gq) * D;
+    const T* p = static_cast<const T*>(a.query.p) + (uint64_t)(s.row0 + ri / gq) * a.query.stride + (uint64_t)(head * gq + ri % gq) * a.query.pitch;
     qs[rr * kQueryPitch + d] = d < D ? (float)p[d] : 0.f;
   }
   __syncthreads();
@@ -322,11 +321,6 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
       bool inside = true;  // every row sees every token of the turn
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) inside &= held[b] && block[b] >= all_from && block[b] < all_to;
-      // ---- logits of eight tokens per lane: 16 half + 4 q + i
-      wave_fence();
-#pragma unroll
-      for (int b = 0; b < BLOCKS; ++b) put_key_pairs(b, kp[b]);
-      wave_fence();
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) {
         const f32x4* from = reinterpret_cast<const f32x4*>(rec[b] + g.vparams_at + inner[b] * (kPagedBlock * 2) * ncg);
@@ -334,6 +328,11 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
         for (int i = 0; i < kValueLoads; ++i) vp[b][i] = from[vget[i]];
         load_words(vc[b], rec[b] + g.vcodes_at + inner[b] * (DP * BITS) + lane * LW);
       }
+      // ---- logits of eight tokens per lane: 16 half + 4 q + i
+      wave_fence();
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b) put_key_pairs(b, kp[b]);
+      wave_fence();
       __builtin_amdgcn_sched_barrier(0);  // phases one after the other: interleaved, they want more registers than there are
       float x[8];
       uint32_t unseen = 0;  // bit j: this lane's row does not see its token j
@@ -480,9 +479,12 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
   } else {
     // ---- the last blocks, one at a time, in the columns of group 0
     typedef typename Row<T>::Frag Frag;
-    constexpr uint32_t kTilePitch = tile_pitch<T>();
-    T* tile = reinterpret_cast<T*>(own);  // [32][kTilePitch]
-    const bool wvec = D * sizeof(T) % 16 == 0;
+    constexpr uint32_t kTilePitch = tile_pitch<T>(S);
+    T* tile = reinterpret_cast<T*>(own);  // values [32][kTilePitch]
+    const uint32_t DW = g.DW;
+    // rows at one position see the same tokens, and what none sees is not read: nothing to keep apart
+    const bool apart = s.m > 1;
+    const int64_t first_left = a.window != 0 ? w.total - s.m + row0 / gq - (int64_t)a.window : -1;
 #pragma unroll 1
     for (uint32_t i = part.tail_at + wave; i < w.tiles; i += 4) {
       const uint32_t block = block_at(w, i);
@@ -492,129 +494,136 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
       const int kend = clamped(kq - t0, 0, 32), vend = clamped(vq - t0, 0, 32), end = clamped(w.hi - t0, 0, 32);
       const int see_to = group == 0 ? clamped(pos - t0, -1, 31) : -1, see_from = clamped(left - t0, -1, 31);
       const int sinks = clamped((int64_t)a.sinks - t0, 0, 32), held = rec != nullptr ? 0 : kend;
+      const int any_from = clamped(first_left - t0, -1, 31);  // no row sees (sinks, any_from]
       const auto seen = [&](int tau) { return tau <= see_to && (tau > see_from || tau < sinks) && tau >= held; };
-      // values that lie as rows, eight lanes a token, 64 channels at a time: fetched while the logits are
-      // computed where the registers hold them
-      constexpr int kChunks = (F + 3) / 4;
-      constexpr bool kAhead = kChunks * sizeof(T) <= 8;
-      Frag values[kAhead ? kChunks : 1][4];
-      const auto load_values = [&](int chunk, Frag(&to)[4]) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int tau = 8 * k + (int)(lane / 8);
-          const uint32_t d = 64 * chunk + lane % 8 * 8;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) to[k][j] = (T)0.f;
-          if (tau >= vend && tau < end && d < D)
-            to[k] = load_frag(row_of<T>(g, a.c.vwin, s, head, t0 + tau, a.values), t0 + tau < s.n ? wvec : a.values.vec != 0, d, D);
-        }
-      };
-      if constexpr (kAhead) {
-#pragma unroll
-        for (int i = 0; i < kChunks; ++i) load_values(i, values[i]);
-      }
-      float x[8];
+      const auto read = [&](int tau) { return tau < end && (tau > any_from || tau < sinks); };
+      // rows: keys as the product reads them (token 16 half + col, channels 8 S q + 8 k), values eight lanes a token
+      Frag k8[2][S];
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int tau = 16 * half + (int)col;
-        const bool packed = tau < kend;
-        const T* p = !packed && tau < end ? row_of<T>(g, a.c.kwin, s, head, t0 + tau, a.keys) : nullptr;
-        const bool vec = t0 + tau < s.n ? wvec : a.keys.vec != 0;
-        const uint32_t* words = rec + inner * (DP * BITS) + lane * LW;
-        const float2* pairs = reinterpret_cast<const float2*>(rec + g.kparams_at) +
-                              quotient(inner * kPagedBlock + tau, G, g.group_magic) * DP + 8 * S * q;
-        Frag k8[S];
+        const bool there = tau >= kend && read(tau);
+        const T* p = there ? row_of<T>(g, a.c.kwin, s, head, t0 + tau, a.keys) : nullptr;
 #pragma unroll
         for (int k = 0; k < S; ++k) {
+          const uint32_t d = 8 * S * q + 8 * k;
+          k8[half][k] = zero_frag<T>();
+          if (there && d < DW) k8[half][k] = load_frag(p, d);
+        }
+      }
+      constexpr int kOctets = 4 * S;                     // of a row
+      constexpr int kPieces = 32 * kOctets / 64;         // of a lane
+      constexpr int kAhead = sizeof(T) * S <= 16 ? kPieces : kPieces / 4;  // fetched before the logits, where registers allow
+      Frag v8[kAhead];
+      uint32_t bad = 0;  // tokens with a value that is not finite: it goes to the rows that see them alone
+      const auto piece = [&](int k, int* tau, uint32_t* d) {
+        const uint32_t u = lane + 64 * k;
+        *tau = (int)(u / kOctets);
+        *d = u % kOctets * 8;
+        return *tau >= vend && read(*tau) && *d < DW;
+      };
+      const auto load_values = [&](int k0) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) k8[k][j] = (T)0.f;
-          if (p != nullptr && 8 * S * q + 8 * k < D) {
-            k8[k] = load_frag(p, vec, 8 * S * q + 8 * k, D);
-          } else if (packed && rec != nullptr) {
+        for (int k = 0; k < kAhead; ++k) {
+          int tau;
+          uint32_t d;
+          const bool there = piece(k0 + k, &tau, &d);
+          v8[k] = zero_frag<T>();
+          if (there) v8[k] = load_frag(row_of<T>(g, a.c.vwin, s, head, t0 + tau, a.values), d);
+        }
+      };
+      const auto put_values = [&](int k0) {
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          int tau;
+          uint32_t d;
+          (void)piece(k0 + k, &tau, &d);
+          if (apart && wild<T>(v8[k])) {
+            bad |= 1u << tau;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v8[k][j] = fabsf((float)v8[k][j]) <= kLargest ? v8[k][j] : (T)0.f;
+          }
+          if (tau < vend) continue;
+          u32x4* to = reinterpret_cast<u32x4*>(tile + tau * kTilePitch + d);
+          const u32x4* from = reinterpret_cast<const u32x4*>(&v8[k]);
+          to[0] = from[0];
+          if constexpr (sizeof(T) == 4) to[1] = from[1];
+        }
+      };
+      load_values(0);
+      // packed keys among them
+      if (kend > 0) {
+        const uint32_t* from = rec != nullptr ? rec : a.c.pages;
+        const uint32_t* words = from + inner * (DP * BITS) + lane * LW;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int tau = 16 * half + (int)col;
+          const float2* pairs = reinterpret_cast<const float2*>(from + g.kparams_at) +
+                                quotient(inner * kPagedBlock + tau, G, g.group_magic) * DP + 8 * S * q;
+#pragma unroll
+          for (int k = 0; k < S; ++k) {
+            if (tau >= kend) continue;
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-              k8[k][j] = (T)decoded<T>(words[paged_word(BITS, half * S + k, j)] >> paged_bit(BITS, half * S + k, j) & ((1u << BITS) - 1),
-                                       pairs[8 * k + j]);
+              k8[half][k][j] = (T)decoded<T>(words[paged_word(BITS, half * S + k, j)] >> paged_bit(BITS, half * S + k, j) & ((1u << BITS) - 1),
+                                             pairs[8 * k + j]);
           }
+          __builtin_amdgcn_sched_barrier(0);
         }
-        f32x4 c = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < S; ++k) {
-          Frag q8;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) q8[j] = (T)qrow[8 * k + j];
-          c = mul16(k8[k], q8, c);
-        }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) x[4 * half + k] = seen(16 * half + 4 * (int)q + k) ? c[k] * scale : -INFINITY;
-        __builtin_amdgcn_sched_barrier(0);
       }
+      f32x4 c[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+      for (int k = 0; k < S; ++k) {
+        Frag q8;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q8[j] = (T)qrow[8 * k + j];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) c[half] = mul16(k8[half][k], q8, c[half]);
+      }
+      float x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = seen(j / 4 * 16 + 4 * (int)q + j % 4) ? c[j / 4][j % 4] * scale : -INFINITY;
       weigh(x);
       Frag p8;
 #pragma unroll
       for (int j = 0; j < 8; ++j) p8[j] = (T)x[j];
-      uint32_t bad = 0;  // tokens with a value that is not finite: it goes to the rows that see them alone
+      wave_fence();
 #pragma unroll
-      for (int f0 = 0; f0 < F; f0 += 4) {
-        if constexpr (!kAhead) load_values(f0 / 4, values[0]);
-        wave_fence();
-        // 32 tokens of 64 channels: eight lanes a token
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int tau = 8 * k + (int)(lane / 8);
-          const uint32_t to = lane % 8 * 8;
-          if (tau < vend) continue;
-          Frag v8 = values[kAhead ? f0 / 4 : 0][k];
+      for (int k0 = 0; k0 < kPieces; k0 += kAhead) {
+        if (k0 > 0) load_values(k0);
+        put_values(k0);
+      }
+      if (vend > 0) {
+        // packed values among them: eight tokens of one channel a lane
+        const uint32_t* from = rec != nullptr ? rec : a.c.pages;
+        const uint32_t* words = from + g.vcodes_at + inner * (DP * BITS) + lane * LW;
+#pragma unroll 2
+        for (int f = 0; f < F; ++f) {
+          const uint32_t d = 16 * f + col;
+          const float2* pairs = reinterpret_cast<const float2*>(from + g.vparams_at) + inner * kPagedBlock * ncg +
+                                quotient(d < D ? d : D - 1, G, g.group_magic);
+          float v[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            if (!(fabsf((float)v8[j]) <= kLargest)) {
-              bad |= 1u << tau;
-              v8[j] = (T)0.f;
-            }
-          if constexpr (sizeof(T) == 4) {
-            reinterpret_cast<f32x4*>(tile + tau * kTilePitch + to)[0] = f32x4{v8[0], v8[1], v8[2], v8[3]};
-            reinterpret_cast<f32x4*>(tile + tau * kTilePitch + to)[1] = f32x4{v8[4], v8[5], v8[6], v8[7]};
-          } else {
-            const uint4 u = __builtin_bit_cast(uint4, v8);
-            reinterpret_cast<uint2*>(tile + tau * kTilePitch + to)[0] = make_uint2(u.x, u.y);
-            reinterpret_cast<uint2*>(tile + tau * kTilePitch + to)[1] = make_uint2(u.z, u.w);
+            v[j] = decoded<T>(words[paged_word(BITS, f, j)] >> paged_bit(BITS, f, j) & ((1u << BITS) - 1),
+                              pairs[(j / 4 * 16 + 4 * q + j % 4) * ncg]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int tau = j / 4 * 16 + 4 * (int)q + j % 4;
+            const bool fine = fabsf(v[j]) <= kLargest, real = d < D && rec != nullptr && read(tau);
+            if (tau >= vend) continue;
+            bad |= apart && real && !fine ? 1u << tau : 0u;
+            tile[tau * kTilePitch + d] = (T)(real && (fine || !apart) ? v[j] : 0.f);
           }
         }
-        if (vend > 0) {
-          // packed ones among them: eight tokens of one channel a lane
+      }
+      wave_fence();
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if (f0 + k >= F) continue;
-            const uint32_t d = 16 * (f0 + k) + col;
-            const uint32_t* from = rec != nullptr ? rec : a.c.pages;
-            const uint32_t* words = from + g.vcodes_at + inner * (DP * BITS) + lane * LW;
-            const float2* pairs = reinterpret_cast<const float2*>(from + g.vparams_at) + inner * kPagedBlock * ncg +
-                                  quotient(d < D ? d : D - 1, G, g.group_magic);
-            float v[8];
+      for (int f = 0; f < F; ++f) {
+        Frag t8;
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-              v[j] = decoded<T>(words[paged_word(BITS, f0 + k, j)] >> paged_bit(BITS, f0 + k, j) & ((1u << BITS) - 1),
-                                pairs[(j / 4 * 16 + 4 * q + j % 4) * ncg]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const int tau = j / 4 * 16 + 4 * (int)q + j % 4;
-              const bool fine = fabsf(v[j]) <= kLargest, real = d < D && rec != nullptr;
-              if (tau >= vend) continue;
-              bad |= real && !fine ? 1u << tau : 0u;
-              tile[tau * kTilePitch + 16 * k + col] = (T)(real && fine ? v[j] : 0.f);
-            }
-          }
-        }
-        wave_fence();
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (f0 + k >= F) continue;
-          Frag v8;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) v8[j] = tile[(j / 4 * 16 + 4 * q + j % 4) * kTilePitch + 16 * k + col];
-          acc[f0 + k] = mul16(v8, p8, acc[f0 + k]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < 8; ++j) t8[j] = tile[(j / 4 * 16 + 4 * q + j % 4) * kTilePitch + 16 * f + col];
+        acc[f] = mul16(t8, p8, acc[f]);
       }
       if (__any(bad != 0)) {
 #pragma unroll
@@ -707,7 +716,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
 template <class T>
 __global__ void __launch_bounds__(256) k_paged_rows_join(PagedAttention a, RowsPlan plan, const float* partial) {
   __shared__ float part_out[4][kPagedMaxHeadDim];
-  __shared__ float2 part_state[4];
+  __shared__ float part_state[4];
   const PagedGeometry& g = a.c.geo;
   const uint32_t head = blockIdx.y, row = blockIdx.x, lane = threadIdx.x % 64, wave = threadIdx.x / 64;
   const PagedSequence s = paged_sequence(a.b, g, blockIdx.z);
@@ -720,26 +729,42 @@ __global__ void __launch_bounds__(256) k_paged_rows_join(PagedAttention a, RowsP
   const uint64_t home = (((uint64_t)blockIdx.z * g.heads + head) * plan.stride + row) * places;
   const float2* states = reinterpret_cast<const float2*>(
       partial + (uint64_t)a.b.sequences * g.heads * plan.stride * places * g.DP);
+  // every wave takes a quarter of the splits, 64 at a time: their factors a lane each, then their outputs
   float top = -INFINITY;
   for (uint32_t k = lane; k < count; k += 64) top = fmaxf(top, states[home + k].x);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
   const float base = top == -INFINITY ? 0.f : top;
+  const uint32_t quarter = (count + 3) / 4, from = wave * quarter, to = from + quarter < count ? from + quarter : count;
   float sum = 0.f, x[kPagedMaxHeadDim / 64] = {0.f};
-#pragma unroll 4
-  for (uint32_t k = wave; k < count; k += 4) {
-    const float2 st = states[home + k];
-    const float f = __builtin_amdgcn_exp2f(st.x - base);
-    sum += f * st.y;
+  for (uint32_t k0 = from; k0 < to; k0 += 64) {
+    const uint32_t n = to - k0 < 64 ? to - k0 : 64;
+    float factor = 0.f;
+    if (lane < n) {
+      const float2 st = states[home + k0 + lane];
+      factor = __builtin_amdgcn_exp2f(st.x - base);
+      sum += factor * st.y;
+    }
 #pragma unroll
-    for (uint32_t j = 0; j < kPagedMaxHeadDim / 64; ++j)
-      if (j * 64 + lane < g.D) x[j] += f * partial[(home + k) * g.DP + j * 64 + lane];
+    for (uint32_t j = 0; j < kPagedMaxHeadDim / 64; ++j) {
+      if (j * 64 >= g.DP) continue;
+      const float* p = partial + (home + k0) * g.DP + (j * 64 + lane < g.DP ? j * 64 + lane : 0);
+      for (uint32_t k = 0; k < n; k += 8) {
+        float v[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) v[i] = p[(uint64_t)(k + i < n ? k + i : n - 1) * g.DP];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) x[j] += __shfl(factor, (int)((k + i) % 64)) * v[i];  // zero from n on
+      }
+    }
   }
 #pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+#pragma unroll
   for (uint32_t j = 0; j < kPagedMaxHeadDim / 64; ++j) part_out[wave][j * 64 + lane] = x[j];
-  if (lane == 0) part_state[wave].x = sum;
+  if (lane == 0) part_state[wave] = sum;
   __syncthreads();
-  sum = part_state[0].x + part_state[1].x + part_state[2].x + part_state[3].x;
+  sum = part_state[0] + part_state[1] + part_state[2] + part_state[3];
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   T* out = static_cast<T*>(a.out) + (uint64_t)(s.row0 + row / gq) * a.out_stride + (uint64_t)(head * gq + row % gq) * g.D;
   for (uint32_t d = threadIdx.x; d < g.D; d += 256)
