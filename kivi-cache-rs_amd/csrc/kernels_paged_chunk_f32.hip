@@ -1,0 +1,9 @@
+// kernels_paged_chunk_f32.hip — attention of long chunks over the paged cache, rows of f32
+// (paged_chunk.hpp).
+#include "paged_chunk.hpp"
+
+namespace kivi {
+
+template hipError_t launch_paged_chunk<float>(const PagedAttention&, const ChunkPlan&, float*, hipStream_t);
+
+}  // namespace kivi

@@ -16,6 +16,15 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
+// What the lanes of a wave wrote to its LDS is there for its other lanes.
+__device__ __forceinline__ void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+__device__ __forceinline__ int clamped(int64_t x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : (int)x; }
+
 // Eight elements of a row.
 template <class T>
 struct Row;
@@ -123,7 +132,7 @@ __device__ float value_of(const PagedAttention& a, const PagedSequence& s, const
   const uint32_t in_page = token_in_page(g, t), tau = in_page % 32, j = tau % 4 + tau / 16 * 4;
   const uint32_t* words = rec + g.vcodes_at + (uint64_t)(in_page / 32) * g.block_words() + (tau % 16 / 4 * 16 + d % 16) * g.lane_words();
   const float2 pair = reinterpret_cast<const float2*>(rec + g.vparams_at)[(uint64_t)in_page * g.ncg + quotient(d, g.G, g.group_magic)];
-  return (float)(T)decoded<T>(words[paged_word(g.bits, d / 16, j)] >> paged_bit(g.bits, d / 16, j) & g.levels(), pair);
+  return decoded<T>(words[paged_word(g.bits, d / 16, j)] >> paged_bit(g.bits, d / 16, j) & g.levels(), pair);
 }
 
 // Chunks of few rows (kernels_paged_rows_*.hip): sequences whose KV heads have more than `over` and at
@@ -146,5 +155,19 @@ __host__ __device__ constexpr int rows_most_blocks(uint32_t bits, uint32_t S) {
 // HALVES: G is an odd multiple of 16 (a block's halves may lie in two groups).
 template <class T, bool HALVES>
 hipError_t launch_paged_rows(const PagedAttention& a, const RowsPlan& p, float* partial, hipStream_t stream);
+
+
+// Longer chunks (kernels_paged_chunk_*.hip): sequences whose KV heads have more than `over` rows.
+struct ChunkPlan {
+  uint32_t over, tile_rows, tile, splits, least;  // rows of a workgroup, tokens of a tile, splits of `least` tiles or a multiple
+};
+// Rows of a workgroup and tokens of a tile by what the registers (512 a lane of one wave, 256 of two) and
+// LDS hold.
+constexpr uint32_t paged_chunk_waves(uint32_t type_bytes, uint32_t S) { return type_bytes == 2 && S <= 4 ? 8 : 4; }
+constexpr uint32_t paged_chunk_tile(uint32_t S) { return S <= 4 ? 64 : 32; }
+inline uint32_t paged_chunk_rows(const PagedGeometry& g) { return 32 * paged_chunk_waves(g.type_bytes(), g.S()); }
+inline uint32_t paged_chunk_tokens(const PagedGeometry& g) { return paged_chunk_tile(g.S()); }
+template <class T>
+hipError_t launch_paged_chunk(const PagedAttention& a, const ChunkPlan& p, float* partial, hipStream_t stream);
 
 }  // namespace kivi

@@ -119,15 +119,6 @@ __host__ __device__ inline uint32_t rows_lds_words(uint32_t S, uint32_t ncg, uin
   return rows * (32 * S + 4) + (pairs > ends ? pairs : ends);
 }
 
-// What the lanes of a wave wrote to its LDS is there for its other lanes.
-__device__ __forceinline__ void wave_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-__device__ __forceinline__ int clamped(int64_t x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : (int)x; }
-
 // How one row tile's walk is cut: blocks whose keys and values are all packed in `mains` splits of `per`
 // (list places), then the last blocks in one of their own.
 struct RowsPart {
@@ -752,7 +743,7 @@ __global__ void __launch_bounds__(256) k_paged_rows_join(PagedAttention a, RowsP
       for (uint32_t k = 0; k < n; k += 8) {
         float v[8];
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) v[i] = p[(uint64_t)(k + i < n ? k + i : n - 1) * g.DP];
+        for (uint32_t i = 0; i < 8; ++i) v[i] = k + i < n ? p[(uint64_t)(k + i) * g.DP] : 0.f;
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i) x[j] += __shfl(factor, (int)((k + i) % 64)) * v[i];  // zero from n on
       }
