@@ -46,7 +46,7 @@ struct Plan {
 // Workgroups that the longest lengths would give: many more than run at once (256 compute units, two or
 // so each), so that ragged lengths even out.
 constexpr uint64_t kRowsWorkgroups = 8192;
-constexpr uint64_t kChunkWorkgroups = 1024;
+constexpr uint64_t kComputeUnits = 256;
 constexpr uint64_t kMostSplits = 512;
 
 Plan plan_of(const PagedGeometry& g, const PagedBatch& b, uint32_t qh, uint64_t window, uint64_t sinks) {
@@ -63,7 +63,11 @@ Plan plan_of(const PagedGeometry& g, const PagedBatch& b, uint32_t qh, uint64_t 
     const uint32_t decode = gq <= 4 ? 4 : gq <= 8 ? 8 : kRowsMost;
     const uint32_t most[2] = {decode, kRowsMost};
     uint32_t over = 0;
+    // Where most sequences have to be near the longest chunk, one launch takes all rows of any number.
+    const bool alike = (uint64_t)b.rows * 2 > (uint64_t)b.sequences * b.max_rows;
     for (uint32_t i = 0; i < 2 && over < rows && over < kRowsMost; ++i) {
+      if (alike && rows > kRowsMost) break;
+      if (alike && rows > most[i]) continue;
       RowsPlan& r = p.rows[p.row_launches];
       r.over = over;
       r.most = most[i];
@@ -79,21 +83,29 @@ Plan plan_of(const PagedGeometry& g, const PagedBatch& b, uint32_t qh, uint64_t 
         r.least = (uint32_t)((least + turn - 1) / turn * turn);
         r.splits = (uint32_t)((blocks + r.least - 1) / r.least);
       };
+      // last blocks: the windows' tokens and the new ones, a block a wave
+      r.tails = (uint32_t)std::min<uint64_t>((g.R + (r.most + gq - 1) / gq + 2 * kPagedBlock - 2) / (4 * kPagedBlock) + 1, 64);
       cut(all, kMostSplits);
       const uint64_t most_splits = r.splits;
       if (tokens < all) cut(tokens, most_splits);
       p.rows_at[p.row_launches++] = p.floats;
-      p.floats += heads * r.stride * (most_splits + 1) * (g.DP + 2);  // and the last blocks
+      p.floats += heads * r.stride * (most_splits + r.tails) * (g.DP + 2);
       over = most[i];
     }
-    p.chunk.over = kRowsMost;
+    p.chunk.over = alike && rows > kRowsMost ? 0 : kRowsMost;
   }
   p.chunks = rows > p.chunk.over;
   p.chunk.tile_rows = paged_chunk_rows(g);
   p.chunk.tile = paged_chunk_tokens(g);
   p.chunk.least = 4;
-  const uint64_t groups = std::max<uint64_t>(1, (uint64_t)b.rows * gq / p.chunk.tile_rows) * g.heads;
-  const uint64_t want = std::min<uint64_t>((kChunkWorkgroups + groups - 1) / groups, 64);
+  const uint64_t groups = std::max<uint64_t>(1, (uint64_t)b.rows * gq / p.chunk.tile_rows) * g.heads;  // about
+  // one workgroup fills a compute unit: the fewest splits whose last round wastes little
+  uint64_t want = 1;
+  double best = 1e30;
+  for (uint64_t n = 1; n <= 64; ++n) {
+    const double rounds = (double)((groups * n + kComputeUnits - 1) / kComputeUnits) / (double)n;
+    if (rounds < 0.85 * best) best = rounds, want = n;
+  }
   const auto chunk_splits = [&](uint64_t n) {
     return (uint32_t)std::max<uint64_t>(1, std::min(want, (n + p.chunk.tile - 1) / p.chunk.tile / p.chunk.least));
   };

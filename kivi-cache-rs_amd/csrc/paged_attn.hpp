@@ -25,6 +25,39 @@ __device__ __forceinline__ void wave_fence() {
 
 __device__ __forceinline__ int clamped(int64_t x, int lo, int hi) { return x < lo ? lo : x > hi ? hi : (int)x; }
 
+// x of the lanes 16 (32) away, as the vector ALU swaps rows: both results together hold every lane's own
+// and its partner's.
+template <int BY>
+__device__ __forceinline__ void swapped(float x, float* a, float* b) {
+  const uint32_t u = __float_as_uint(x);
+  if constexpr (BY == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    *a = __uint_as_float(r[0]), *b = __uint_as_float(r[1]);
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    *a = __uint_as_float(r[0]), *b = __uint_as_float(r[1]);
+  }
+}
+template <int BY>
+__device__ __forceinline__ float sum_with(float x) {
+  float a, b;
+  swapped<BY>(x, &a, &b);
+  return a + b;
+}
+template <int BY>
+__device__ __forceinline__ float max_with(float x) {
+  float a, b;
+  swapped<BY>(x, &a, &b);
+  return fmaxf(a, b);
+}
+// Sum over the lanes of a row of 16 that lie N apart (N 4 or 8), in every lane.
+template <int N>
+__device__ __forceinline__ float sum_row(float x) {
+  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xF, 0xF, true));  // rotated by 8
+  if constexpr (N == 4) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x124, 0xF, 0xF, true));
+  return x;
+}
+
 // Eight elements of a row.
 template <class T>
 struct Row;
@@ -141,8 +174,9 @@ constexpr uint32_t kRowsMost = 32;
 struct RowsPlan {
   uint32_t over, most;     // rows of a KV head that this launch takes
   uint32_t blocks;         // column groups: 4 (up to 4 rows), 2 (8) or 1 (16 rows a tile)
-  uint32_t splits;         // at most this many of a walk,
+  uint32_t splits;         // at most this many of a walk's packed blocks,
   uint32_t least;          // each of a multiple of this many 32-token blocks (itself one of 4 * blocks)
+  uint32_t tails;          // at most this many of its last blocks
   uint32_t stride;         // rows of a (sequence, head) in the partials
 };
 // Whether the kernels of few rows take this cache (else the chunk kernel takes everything).
@@ -155,7 +189,6 @@ __host__ __device__ constexpr int rows_most_blocks(uint32_t bits, uint32_t S) {
 // HALVES: G is an odd multiple of 16 (a block's halves may lie in two groups).
 template <class T, bool HALVES>
 hipError_t launch_paged_rows(const PagedAttention& a, const RowsPlan& p, float* partial, hipStream_t stream);
-
 
 // Longer chunks (kernels_paged_chunk_*.hip): sequences whose KV heads have more than `over` rows.
 struct ChunkPlan {

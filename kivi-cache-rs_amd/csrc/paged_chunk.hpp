@@ -661,41 +661,46 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
   }
 }
 
-// Joins the splits of one row and query head per wave, its lanes over the channels.
+// Joins the splits of 16 rows of one KV head, a row at a time per wave, its lanes over the channels.
+constexpr uint32_t kJoinRows = 16;
 template <class T>
-__global__ void __launch_bounds__(256)
-    k_paged_chunk_join(PagedAttention a, ChunkPlan plan, const float* partial) {
+__global__ void __launch_bounds__(256) k_paged_chunk_join(PagedAttention a, ChunkPlan plan, const float* partial) {
   const PagedGeometry& g = a.c.geo;
   const PagedSequence s = paged_sequence(a.b, g, blockIdx.z);
-  const uint32_t gq = a.qh / g.heads, rows = s.m * gq, lane = threadIdx.x % 64;
-  const uint32_t splits = plan.splits, tile_rows = plan.tile_rows;
-  if (rows <= plan.over) return;
+  const uint32_t gq = a.qh / g.heads, rows = s.m * gq, lane = threadIdx.x % 64, head = blockIdx.x % g.heads;
+  const uint32_t first = blockIdx.x / g.heads * kJoinRows;
+  if (rows <= plan.over || first >= rows) return;
+  const uint32_t r0 = first / plan.tile_rows * plan.tile_rows;
+  const Walk w = walk_of(a, s, r0, r0 + plan.tile_rows < rows ? r0 + plan.tile_rows : rows, gq, plan.tile);
+  const uint32_t count = part_of(w.tiles, plan.splits, plan.least, 0).count;
+  if (count == 1) return;
   const uint64_t all = (uint64_t)a.b.rows * a.qh;
-  for (uint64_t i = (uint64_t)blockIdx.x * 4 + threadIdx.x / 64; i < (uint64_t)s.m * a.qh; i += (uint64_t)gridDim.x * 4) {
-    const uint32_t token = (uint32_t)(i / a.qh), qhead = (uint32_t)(i % a.qh), r = token * gq + qhead % gq;
-    const uint32_t r0 = r / tile_rows * tile_rows;
-    const Walk w = walk_of(a, s, r0, r0 + tile_rows < rows ? r0 + tile_rows : rows, gq, plan.tile);
-    const uint32_t count = part_of(w.tiles, splits, plan.least, 0).count;
-    if (count == 1) continue;
-    const uint64_t place = (uint64_t)s.row0 * a.qh + i;
-    const float2* state = reinterpret_cast<const float2*>(partial + splits * all * g.DP);
-    float top = -INFINITY;
-    for (uint32_t k = 0; k < count; ++k) top = fmaxf(top, state[k * all + place].x);
-    const float base = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, x[kPagedMaxHeadDim / 64] = {0.f};
-    for (uint32_t k = 0; k < count; ++k) {
-      const float2 st = state[k * all + place];
-      const float f = __builtin_amdgcn_exp2f(st.x - base);
-      sum += f * st.y;
+  const float2* state = reinterpret_cast<const float2*>(partial + plan.splits * all * g.DP);
+  for (uint32_t r = first + threadIdx.x / 64; r < first + kJoinRows && r < rows; r += 4) {
+    const uint32_t token = r / gq, qhead = head * gq + r % gq;
+    const uint64_t place = (uint64_t)(s.row0 + token) * a.qh + qhead;
+    const float2 mine = lane < count ? state[lane * all + place] : make_float2(-INFINITY, 0.f);  // at most 64 splits
+    float top = mine.x;
 #pragma unroll
-      for (uint32_t j = 0; j < kPagedMaxHeadDim / 64; ++j)
-        if (j * 64 + lane < g.D) x[j] += f * partial[(k * all + place) * g.DP + j * 64 + lane];
-    }
+    for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    const float factor = __builtin_amdgcn_exp2f(mine.x - (top == -INFINITY ? 0.f : top));
+    float sum = factor * mine.y;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     T* out = static_cast<T*>(a.out) + (uint64_t)(s.row0 + token) * a.out_stride + (uint64_t)qhead * g.D;
+    for (uint32_t d = lane; d < (g.D + 63) / 64 * 64; d += 64) {
+      const float* p = partial + place * g.DP + (d < g.DP ? d : 0);
+      float x = 0.f;
+      for (uint32_t k = 0; k < count; k += 4) {
+        float v[4];
 #pragma unroll
-    for (uint32_t j = 0; j < kPagedMaxHeadDim / 64; ++j)
-      if (j * 64 + lane < g.D) out[j * 64 + lane] = (T)(x[j] * inv);
+        for (uint32_t i = 0; i < 4; ++i) v[i] = k + i < count ? p[(k + i) * all * g.DP] : 0.f;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) x += __shfl(factor, (int)(k + i) % 64) * v[i];
+      }
+      if (d < g.D) out[d] = (T)(x * inv);
+    }
   }
 }
 
@@ -711,7 +716,7 @@ hipError_t chunk_launch(const PagedAttention& a, const ChunkPlan& p, float* part
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(kernel, dim3((uint32_t)x, 1, a.b.sequences), dim3(WAVES * 64), bytes, stream, a, p, partial);
   if (p.splits > 1) {
-    const uint64_t joins = std::min<uint64_t>(((uint64_t)a.b.max_rows * a.qh + 3) / 4, 1u << 16);
+    const uint64_t joins = (rows + kJoinRows - 1) / kJoinRows * g.heads;
     hipLaunchKernelGGL(k_paged_chunk_join<T>, dim3((uint32_t)joins, 1, a.b.sequences), dim3(256), 0, stream, a, p, partial);
   }
   return hipGetLastError();

@@ -119,20 +119,49 @@ __host__ __device__ inline uint32_t rows_lds_words(uint32_t S, uint32_t ncg, uin
   return rows * (32 * S + 4) + (pairs > ends ? pairs : ends);
 }
 
-// How one row tile's walk is cut: blocks whose keys and values are all packed in `mains` splits of `per`
-// (list places), then the last blocks in one of their own.
+// A lane's N code words.
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&words)[N], const uint32_t* from) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const u32x4 x = reinterpret_cast<const u32x4*>(from)[i];
+      words[4 * i] = x[0], words[4 * i + 1] = x[1], words[4 * i + 2] = x[2], words[4 * i + 3] = x[3];
+    }
+  } else if constexpr (N % 2 == 0) {
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const uint2 x = reinterpret_cast<const uint2*>(from)[i];
+      words[2 * i] = x.x, words[2 * i + 1] = x.y;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) words[i] = from[i];
+  }
+}
+
+// How one row tile's walk is cut: the places [0, main_to) of its list of blocks have packed values and go to
+// `mains` splits of `per`; the places from tail_at on have values that are rows and go to `tails` splits of
+// `tail_per`. A block that has both is in both: the splits see its packed tokens, and its rows.
 struct RowsPart {
-  uint32_t tail_at, per, mains, count;
+  uint32_t main_to, tail_at, per, mains, tail_per, tails, count;
 };
+__device__ __forceinline__ uint32_t place_of(const Walk& w, uint32_t block) {
+  const uint32_t p = block < w.head_tiles ? block : w.head_tiles + (block > w.first_tile ? block - w.first_tile : 0);
+  return p < w.tiles ? p : w.tiles;
+}
 __device__ __forceinline__ RowsPart rows_part(const Walk& w, int64_t vq, const RowsPlan& plan) {
   RowsPart p;
-  const uint32_t tail = (uint32_t)(vq / kPagedBlock);  // the first block with a value that is not packed
-  p.tail_at = tail < w.head_tiles ? tail : w.head_tiles + (tail > w.first_tile ? tail - w.first_tile : 0);
-  p.tail_at = p.tail_at < w.tiles ? p.tail_at : w.tiles;
-  p.per = (p.tail_at + plan.splits - 1) / plan.splits;
+  p.main_to = place_of(w, (uint32_t)((vq + kPagedBlock - 1) / kPagedBlock));
+  p.tail_at = place_of(w, (uint32_t)(vq / kPagedBlock));
+  p.per = (p.main_to + plan.splits - 1) / plan.splits;
   p.per = (p.per + plan.least - 1) / plan.least * plan.least;
-  p.mains = p.tail_at == 0 ? 0 : (p.tail_at + p.per - 1) / p.per;
-  p.count = p.mains + (p.tail_at < w.tiles || p.mains == 0 ? 1 : 0);
+  p.mains = p.main_to == 0 ? 0 : (p.main_to + p.per - 1) / p.per;
+  const uint32_t last = w.tiles - p.tail_at;
+  p.tail_per = ((last + plan.tails - 1) / plan.tails + 3) / 4 * 4;  // a block a wave, or as few as the plan has room for
+  p.tails = last == 0 ? 0 : (last + p.tail_per - 1) / p.tail_per;
+  if (p.mains + p.tails == 0) p.tails = 1, p.tail_per = 4;  // nothing seen: zeros
+  p.count = p.mains + p.tails;
   return p;
 }
 __device__ __forceinline__ uint32_t block_at(const Walk& w, uint32_t place) {
@@ -156,17 +185,18 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
   const PagedSequence s = paged_sequence(a.b, g, blockIdx.z);
   const uint32_t gq = a.qh / g.heads, rows = s.m * gq;
   if (rows <= plan.over || rows > plan.most) return;
-  const uint32_t row0 = blockIdx.x / (plan.splits + 1) * ROWS;
+  const uint32_t places = plan.splits + plan.tails;
+  const uint32_t row0 = blockIdx.x / places * ROWS;
   if (row0 >= rows) return;
   const uint32_t row1 = row0 + ROWS < rows ? row0 + ROWS : rows;
   const Walk w = walk_of(a, s, row0, row1, gq, kPagedBlock);
   const int64_t kq = paged_kq(g, s.n), vq = paged_vq(g, s.n);
   const RowsPart part = rows_part(w, vq, plan);
-  // the last blocks take longest and come first
-  const uint32_t turn = blockIdx.x % (plan.splits + 1);
-  const bool tail = turn == 0;
-  if (tail ? part.count == part.mains : turn > part.mains) return;
-  const uint32_t split = tail ? part.mains : turn - 1;
+  // the last blocks first: their chain of loads is the longest
+  const uint32_t turn = blockIdx.x % places;
+  const bool tail = turn < plan.tails;
+  if (tail ? turn >= part.tails : turn - plan.tails >= part.mains) return;
+  const uint32_t split = tail ? part.mains + turn : turn - plan.tails;
 
   const uint32_t D = g.D, G = g.G, ncg = g.ncg, per = G / 16;
   const uint32_t row = row0 + r < rows ? row0 + r : rows - 1;
@@ -198,8 +228,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
     float peak = x[0];
 #pragma unroll
     for (int j = 1; j < 8; ++j) peak = fmaxf(peak, x[j]);
-    peak = fmaxf(peak, __shfl_xor(peak, 16));
-    peak = fmaxf(peak, __shfl_xor(peak, 32));
+    peak = max_with<32>(max_with<16>(peak));
     const float next = fmaxf(top, peak);
     const float base = next == -INFINITY ? 0.f : next;
     const float shrink = __builtin_amdgcn_exp2f(top - base);
@@ -223,10 +252,11 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
     float* kpairs = own;                              // [BLOCKS][4][kKeyPitch]
     float* vpairs = kpairs + BLOCKS * 4 * kKeyPitch;  // [BLOCKS][8][value_pitch] + 16
     const uint32_t vpitch = value_pitch(ncg), vblock = value_block(ncg);
-    const uint32_t to = split * part.per + part.per < part.tail_at ? split * part.per + part.per : part.tail_at;
+    const uint32_t to = split * part.per + part.per < part.main_to ? split * part.per + part.per : part.main_to;
     // every row sees the blocks [all_from, all_to)
     const int64_t first_pos = w.total - s.m + row0 / gq, last_left = a.window != 0 ? w.hi - 1 - (int64_t)a.window : -1;
-    const uint32_t all_to = first_pos < 0 ? 0 : (uint32_t)((first_pos + 1) / kPagedBlock);
+    const int64_t all_end = first_pos + 1 < vq ? first_pos + 1 : vq;
+    const uint32_t all_to = all_end < 0 ? 0 : (uint32_t)(all_end / kPagedBlock);
     const uint32_t all_from = last_left < 0 ? 0 : (uint32_t)((last_left + kPagedBlock) / kPagedBlock);
     // this lane's float4s of a block's pairs, and where their words go in LDS; lanes past the end take the last
     uint32_t kget[kKeyLoads], kput[kKeyLoads], vget[kValueLoads], vput[kValueLoads];
@@ -266,24 +296,6 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
     };
     uint32_t kc[BLOCKS][LW], vc[BLOCKS][LW];
     f32x4 kp[BLOCKS][kKeyLoads], vp[BLOCKS][kValueLoads];
-    const auto load_words = [&](uint32_t(&words)[LW], const uint32_t* from) {
-      if constexpr (LW % 4 == 0) {
-#pragma unroll
-        for (int i = 0; i < LW / 4; ++i) {
-          const uint4 x = reinterpret_cast<const uint4*>(from)[i];
-          words[4 * i] = x.x, words[4 * i + 1] = x.y, words[4 * i + 2] = x.z, words[4 * i + 3] = x.w;
-        }
-      } else if constexpr (LW % 2 == 0) {
-#pragma unroll
-        for (int i = 0; i < LW / 2; ++i) {
-          const uint2 x = reinterpret_cast<const uint2*>(from)[i];
-          words[2 * i] = x.x, words[2 * i + 1] = x.y;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < LW; ++i) words[i] = from[i];
-      }
-    };
     const auto load_key_pairs = [&](f32x4(&pairs)[kKeyLoads], const uint32_t* record, uint32_t in_page) {
       const f32x4* from = reinterpret_cast<const f32x4*>(record + g.kparams_at + quotient(in_page, G, g.group_magic) * (DP * 2));
 #pragma unroll
@@ -293,7 +305,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
 #pragma unroll
       for (int b = 0; b < BLOCKS; ++b) {
         load_key_pairs(kp[b], rec[b], inner[b] * kPagedBlock);
-        load_words(kc[b], rec[b] + inner[b] * (DP * BITS) + lane * LW);
+        load_words<LW>(kc[b], rec[b] + inner[b] * (DP * BITS) + lane * LW);
       }
     };
     const auto put_key_pairs = [&](int b, const f32x4(&from)[kKeyLoads]) {
@@ -317,7 +329,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
         const f32x4* from = reinterpret_cast<const f32x4*>(rec[b] + g.vparams_at + inner[b] * (kPagedBlock * 2) * ncg);
 #pragma unroll
         for (int i = 0; i < kValueLoads; ++i) vp[b][i] = from[vget[i]];
-        load_words(vc[b], rec[b] + g.vcodes_at + inner[b] * (DP * BITS) + lane * LW);
+        load_words<LW>(vc[b], rec[b] + g.vcodes_at + inner[b] * (DP * BITS) + lane * LW);
       }
       // ---- logits of eight tokens per lane: 16 half + 4 q + i
       wave_fence();
@@ -347,8 +359,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
             }
             __builtin_amdgcn_sched_barrier(0);
           }
-          qz += __shfl_xor(qz, 16);
-          qz += __shfl_xor(qz, 32);
+          qz = sum_with<32>(sum_with<16>(qz));
         };
         fold();
         __builtin_amdgcn_sched_barrier(0);
@@ -398,7 +409,8 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
           t0 = group == b ? (int64_t)block[b] * kPagedBlock : t0;
           there = group == b ? held[b] : there;
         }
-        const int see_to = there ? clamped(pos - t0, -1, 31) : -1, see_from = clamped(left - t0, -1, 31);
+        const int64_t last = pos < vq - 1 ? pos : vq - 1;  // packed tokens alone
+        const int see_to = there ? clamped(last - t0, -1, 31) : -1, see_from = clamped(left - t0, -1, 31);
         const int sinks = clamped((int64_t)a.sinks - t0, 0, 32);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -476,18 +488,21 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
     // rows at one position see the same tokens, and what none sees is not read: nothing to keep apart
     const bool apart = s.m > 1;
     const int64_t first_left = a.window != 0 ? w.total - s.m + row0 / gq - (int64_t)a.window : -1;
+    const uint32_t to = part.tail_at + (turn + 1) * part.tail_per < w.tiles ? part.tail_at + (turn + 1) * part.tail_per : w.tiles;
 #pragma unroll 1
-    for (uint32_t i = part.tail_at + wave; i < w.tiles; i += 4) {
+    for (uint32_t i = part.tail_at + turn * part.tail_per + wave; i < to; i += 4) {
       const uint32_t block = block_at(w, i);
       const int64_t t0 = (int64_t)block * kPagedBlock;
       const uint32_t page = quotient(block, g.page_blocks, g.page_magic), inner = block - page * g.page_blocks;
       const uint32_t* rec = t0 < kq ? paged_record_of(a.c, a.b, s, head, page) : nullptr;
       const int kend = clamped(kq - t0, 0, 32), vend = clamped(vq - t0, 0, 32), end = clamped(w.hi - t0, 0, 32);
       const int see_to = group == 0 ? clamped(pos - t0, -1, 31) : -1, see_from = clamped(left - t0, -1, 31);
-      const int sinks = clamped((int64_t)a.sinks - t0, 0, 32), held = rec != nullptr ? 0 : kend;
+      const int sinks = clamped((int64_t)a.sinks - t0, 0, 32);
+      // the splits of packed blocks have the tokens in front of vend; keys of no page are seen by none
+      const int held = rec != nullptr || kend < vend ? vend : kend;
       const int any_from = clamped(first_left - t0, -1, 31);  // no row sees (sinks, any_from]
       const auto seen = [&](int tau) { return tau <= see_to && (tau > see_from || tau < sinks) && tau >= held; };
-      const auto read = [&](int tau) { return tau < end && (tau > any_from || tau < sinks); };
+      const auto read = [&](int tau) { return tau >= vend && tau < end && (tau > any_from || tau < sinks); };
       // rows: keys as the product reads them (token 16 half + col, channels 8 S q + 8 k), values eight lanes a token
       Frag k8[2][S];
 #pragma unroll
@@ -511,7 +526,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
         const uint32_t u = lane + 64 * k;
         *tau = (int)(u / kOctets);
         *d = u % kOctets * 8;
-        return *tau >= vend && read(*tau) && *d < DW;
+        return read(*tau) && *d < DW;
       };
       const auto load_values = [&](int k0) {
 #pragma unroll
@@ -534,7 +549,6 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
 #pragma unroll
             for (int j = 0; j < 8; ++j) v8[k][j] = fabsf((float)v8[k][j]) <= kLargest ? v8[k][j] : (T)0.f;
           }
-          if (tau < vend) continue;
           u32x4* to = reinterpret_cast<u32x4*>(tile + tau * kTilePitch + d);
           const u32x4* from = reinterpret_cast<const u32x4*>(&v8[k]);
           to[0] = from[0];
@@ -545,22 +559,29 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
       // packed keys among them
       if (kend > 0) {
         const uint32_t* from = rec != nullptr ? rec : a.c.pages;
-        const uint32_t* words = from + inner * (DP * BITS) + lane * LW;
+        uint32_t code[LW];
+        load_words<LW>(code, from + inner * (DP * BITS) + lane * LW);
+        const f32x4* pairs = reinterpret_cast<const f32x4*>(from + g.kparams_at) + 4 * S * q;
+        const uint32_t group0 = quotient(inner * kPagedBlock, G, g.group_magic);
+        const uint32_t group1 = HALVES ? quotient(inner * kPagedBlock + 16, G, g.group_magic) : group0;
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const int tau = 16 * half + (int)col;
-          const float2* pairs = reinterpret_cast<const float2*>(from + g.kparams_at) +
-                                quotient(inner * kPagedBlock + tau, G, g.group_magic) * DP + 8 * S * q;
+        for (int k = 0; k < S; ++k) {
+          f32x4 p[2][4];
 #pragma unroll
-          for (int k = 0; k < S; ++k) {
-            if (tau >= kend) continue;
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              k8[half][k][j] = (T)decoded<T>(words[paged_word(BITS, half * S + k, j)] >> paged_bit(BITS, half * S + k, j) & ((1u << BITS) - 1),
-                                             pairs[8 * k + j]);
+          for (int j = 0; j < 4; ++j) {
+            p[0][j] = pairs[group0 * (DP / 2) + 4 * k + j];
+            p[1][j] = HALVES ? pairs[group1 * (DP / 2) + 4 * k + j] : p[0][j];
           }
-          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const bf16x8 c = codes_of<BITS>(code, half * S + k);
+            Frag f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] = (T)fmaf((float)c[j], p[half][j / 2][j % 2 * 2], p[half][j / 2][j % 2 * 2 + 1]);
+            if (16 * half + (int)col < kend) k8[half][k] = f;
+          }
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
       f32x4 c[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
@@ -583,30 +604,6 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
       for (int k0 = 0; k0 < kPieces; k0 += kAhead) {
         if (k0 > 0) load_values(k0);
         put_values(k0);
-      }
-      if (vend > 0) {
-        // packed values among them: eight tokens of one channel a lane
-        const uint32_t* from = rec != nullptr ? rec : a.c.pages;
-        const uint32_t* words = from + g.vcodes_at + inner * (DP * BITS) + lane * LW;
-#pragma unroll 2
-        for (int f = 0; f < F; ++f) {
-          const uint32_t d = 16 * f + col;
-          const float2* pairs = reinterpret_cast<const float2*>(from + g.vparams_at) + inner * kPagedBlock * ncg +
-                                quotient(d < D ? d : D - 1, G, g.group_magic);
-          float v[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            v[j] = decoded<T>(words[paged_word(BITS, f, j)] >> paged_bit(BITS, f, j) & ((1u << BITS) - 1),
-                              pairs[(j / 4 * 16 + 4 * q + j % 4) * ncg]);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int tau = j / 4 * 16 + 4 * (int)q + j % 4;
-            const bool fine = fabsf(v[j]) <= kLargest, real = d < D && rec != nullptr && read(tau);
-            if (tau >= vend) continue;
-            bad |= apart && real && !fine ? 1u << tau : 0u;
-            tile[tau * kTilePitch + d] = (T)(real && (fine || !apart) ? v[j] : 0.f);
-          }
-        }
       }
       wave_fence();
 #pragma unroll
@@ -644,16 +641,14 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
   }
 
   // ---- the columns of a row, over groups and waves
-  sum += __shfl_xor(sum, 16);
-  sum += __shfl_xor(sum, 32);
-  float z = 0.f;
+  sum = sum_with<32>(sum_with<16>(sum));
+  if (!tail) {
+    float z = 0.f;
 #pragma unroll
-  for (int f = 0; f < F; ++f) {
-    float next = zacc[f];
-    next += __shfl_xor(next, 16);
-    next += __shfl_xor(next, 32);
-    z = f % per == 0 ? next : z;
-    acc[f] += z;
+    for (int f = 0; f < F; ++f) {
+      z = f % per == 0 ? sum_with<32>(sum_with<16>(zacc[f])) : z;
+      acc[f] += z;
+    }
   }
   __syncthreads();  // the waves' LDS is done with
   float* outs = lds + ROWS * kQueryPitch;                           // [4][ROWS][DP]
@@ -676,15 +671,12 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
   for (int f = 0; f < F; ++f) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      float v = acc[f][i] * factor;
-#pragma unroll
-      for (int o = ROWS; o < 16; o <<= 1) v += __shfl_xor(v, o);
-      acc[f][i] = v;
+      acc[f][i] *= factor;
+      if constexpr (ROWS < 16) acc[f][i] = sum_row<ROWS>(acc[f][i]);
     }
     if (group == 0) *reinterpret_cast<f32x4*>(outs + (wave * ROWS + r) * DP + 16 * f + 4 * q) = acc[f];
   }
   const uint64_t home = ((uint64_t)blockIdx.z * g.heads + head) * plan.stride;
-  const uint32_t places = plan.splits + 1;
   float2* states = reinterpret_cast<float2*>(partial + (uint64_t)a.b.sequences * g.heads * plan.stride * places * DP);
   if (part.count > 1 && tid < ROWS && row0 + tid < rows) states[(home + row0 + tid) * places + split] = make_float2(all, total);
   if (tid < ROWS) inverse[tid] = total == 0.f ? 0.f : 1.f / total;  // lane r of wave 0: row r
@@ -715,7 +707,7 @@ __global__ void __launch_bounds__(256) k_paged_rows_join(PagedAttention a, RowsP
   if (rows <= plan.over || rows > plan.most || row >= rows) return;
   const uint32_t tile = 16 / plan.blocks, row0 = row / tile * tile;
   const Walk w = walk_of(a, s, row0, row0 + tile < rows ? row0 + tile : rows, gq, kPagedBlock);
-  const uint32_t count = rows_part(w, paged_vq(g, s.n), plan).count, places = plan.splits + 1;
+  const uint32_t count = rows_part(w, paged_vq(g, s.n), plan).count, places = plan.splits + plan.tails;
   if (count == 1) return;
   const uint64_t home = (((uint64_t)blockIdx.z * g.heads + head) * plan.stride + row) * places;
   const float2* states = reinterpret_cast<const float2*>(
@@ -771,7 +763,7 @@ hipError_t rows_launch(const PagedAttention& a, const RowsPlan& p, float* partia
   if (e != hipSuccess) return e;
   constexpr uint32_t kTile = 16 / BLOCKS;
   const uint32_t tiles = (p.stride + kTile - 1) / kTile;
-  hipLaunchKernelGGL(kernel, dim3(tiles * (p.splits + 1), g.heads, a.b.sequences), dim3(256), bytes, stream, a, p, partial);
+  hipLaunchKernelGGL(kernel, dim3(tiles * (p.splits + p.tails), g.heads, a.b.sequences), dim3(256), bytes, stream, a, p, partial);
   hipLaunchKernelGGL(k_paged_rows_join<T>, dim3(p.stride, g.heads, a.b.sequences), dim3(256), 0, stream, a, p, partial);
   return hipGetLastError();
 }
