@@ -424,9 +424,11 @@ __global__ void __launch_bounds__(kThreads)
 // One wave per (sequence, 32-token block, head): codes become rows. A lane takes an octet of channels of
 // eight tokens: of keys a word or two each, of values those of the eight lanes that have its channels, so
 // that rows go out in whole pieces and nothing has to turn over. Tokens that the cache does not hold (at
-// or behind its length, or in a page or slot outside the pool) read as zeros. Bound by the rows it writes.
-template <class T, int BITS>
-__global__ void __launch_bounds__(kThreads)
+// or behind its length, or in a page or slot outside the pool) read as zeros. Bound by the rows it writes;
+// single tokens by latency, of which fetching the code is a good part: VEC (whole octets on 16 bytes) has
+// no stores of single elements in it.
+template <class T, int BITS, bool VEC>
+__global__ void __launch_bounds__(kThreads, 4)
     k_paged_read(PagedView c, PagedBatch b, const int32_t* first, PagedRows keys, PagedRows values, uint32_t S_magic, uint32_t oct_magic) {
   const PagedGeometry& g = c.geo;
   const uint32_t lane = threadIdx.x % 64;
@@ -449,33 +451,27 @@ __global__ void __launch_bounds__(kThreads)
   if (!held) rec = c.pages;  // read, and dropped
   const uint32_t* kcodes = rec + (uint64_t)(in_page / kPagedBlock) * g.block_words();
   const uint32_t* vcodes = kcodes + g.vcodes_at;
-  const uint64_t window = ((uint64_t)(s.slot < 0 ? 0 : s.slot) * g.heads + head) * 2 * g.R;
-
-  // The unit's row of token tau, decoded into x; where that is not packed, its window row or zeros.
-  const auto put = [&](const PagedRows& rows, const void* win, int packed, int tau, uint32_t d, float(&x)[8]) {
-    if (tau < lo || tau >= hi) return;
-    T* to = static_cast<T*>(const_cast<void*>(rows.p)) + (uint64_t)(s.row0 + (base - f0) + tau) * rows.stride + (uint64_t)head * rows.pitch + d;
-    if (tau >= packed && tau < nend) {
-      copy8(static_cast<const T*>(win) + (window + ring_row(g, base + tau)) * g.DW + d, to, rows.vec != 0, D - d);
-      return;
-    }
-    if (!held || tau >= nend) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = 0.f;
-    }
-    store8(to, rows.vec != 0, D - d, x);
-  };
+  const int64_t row0 = s.row0 + (base - f0);  // of the block's first token
 
   for (uint32_t u = lane; u < 16 * S; u += 64) {
     const uint32_t p = quotient(u, oct, oct_magic), o = u - p * oct, d = 8 * o;
     if (d >= D) continue;
+    const auto put = [&](T* to, uint32_t vec, float(&x)[8]) {
+      if (!held) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = 0.f;
+      }
+      store8(to, VEC || vec != 0, VEC ? 8 : D - d, x);
+    };
+    // of keys tokens p + 4 i, of values 4 p + i and 16 + 4 p + i
+    T* kout = static_cast<T*>(const_cast<void*>(keys.p)) + (row0 + p) * (int64_t)keys.stride + (uint64_t)head * keys.pitch + d;
+    T* vout = static_cast<T*>(const_cast<void*>(values.p)) + (uint64_t)head * values.pitch + d;
     uint32_t kwords[8][2], vwords[8][2];
     f32x4 kpairs[4];
     f32x2 vpairs[8];
     const uint32_t q = quotient(o, S, S_magic), k = o - q * S, f = o / 2, group = quotient(in_page, G, g.group_magic);
     const f32x4* pairs = reinterpret_cast<const f32x4*>(rec + g.kparams_at + 2 * d);
     const f32x2* vp = reinterpret_cast<const f32x2*>(rec + g.vparams_at) + (uint64_t)in_page * ncg;
-    const uint32_t cg = quotient(d, G, g.group_magic);
     if (kend > 0) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) kpairs[i] = pairs[group * (g.DP / 2) + i];
@@ -483,35 +479,71 @@ __global__ void __launch_bounds__(kThreads)
       for (uint32_t i = 0; i < 8; ++i) fragment_words<BITS>(kcodes + (q * 16 + p + 4 * (i % 4)) * LW, i / 4 * S + k, kwords[i]);
     }
     if (vend > 0) {
+      const uint32_t cg = quotient(d, G, g.group_magic);
 #pragma unroll
       for (uint32_t j = 0; j < 8; ++j) vpairs[j] = vp[(j / 4 * 16 + 4 * p + j % 4) * ncg + cg];
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) fragment_words<BITS>(vcodes + (p * 16 + 8 * (o % 2) + i) * LW, f, vwords[i]);
     }
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-      const uint32_t tau = p + 4 * i;
-      if (G % kPagedBlock != 0 && kend > 0) {
-        const uint32_t mine = quotient(in_page + tau, G, g.group_magic);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) kpairs[j] = pairs[mine * (g.DP / 2) + j];
-      }
-      float x[8];
-#pragma unroll
-      for (uint32_t j = 0; j < 8; ++j) x[j] = decoded(code_in<BITS>(kwords[i], j), make_float2(kpairs[j / 2][j % 2 * 2], kpairs[j / 2][j % 2 * 2 + 1]));
-      put(keys, c.kwin, kend, (int)tau, d, x);
-    }
-#pragma unroll
-    for (uint32_t j = 0; j < 8; ++j) {
-      const uint32_t tau = j / 4 * 16 + 4 * p + j % 4;
-      float x[8];
+    if (kend > 0) {
 #pragma unroll
       for (uint32_t i = 0; i < 8; ++i) {
-        f32x2 pair = vpairs[j];
-        if (G % 8 != 0 && vend > 0) pair = vp[tau * ncg + quotient(d + i < D ? d + i : D - 1, G, g.group_magic)];
-        x[i] = decoded(code_in<BITS>(vwords[i], j), make_float2(pair.x, pair.y));
+        const int tau = (int)(p + 4 * i);
+        if (G % kPagedBlock != 0) {
+          const uint32_t mine = quotient(in_page + tau, G, g.group_magic);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) kpairs[j] = pairs[mine * (g.DP / 2) + j];
+        }
+        float x[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) x[j] = decoded(code_in<BITS>(kwords[i], j), make_float2(kpairs[j / 2][j % 2 * 2], kpairs[j / 2][j % 2 * 2 + 1]));
+        if (tau >= lo && tau < hi && tau < kend) put(kout + i * 4 * keys.stride, keys.vec, x);
       }
-      put(values, c.vwin, vend, (int)tau, d, x);
+    }
+    if (vend > 0) {
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        const int tau = (int)(j / 4 * 16 + 4 * p + j % 4);
+        float x[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+          f32x2 pair = vpairs[j];
+          if (!VEC && G % 8 != 0) pair = vp[tau * ncg + quotient(d + i < D ? d + i : D - 1, G, g.group_magic)];
+          x[i] = decoded(code_in<BITS>(vwords[i], j), make_float2(pair.x, pair.y));
+        }
+        if (tau >= lo && tau < hi && tau < vend) put(vout + (row0 + tau) * (int64_t)values.stride, values.vec, x);
+      }
+    }
+    if (vend < (int)kPagedBlock) {
+      // window rows, and zeros behind the cache: all fetched, then all written
+      const uint64_t window = ((uint64_t)(s.slot < 0 ? 0 : s.slot) * g.heads + head) * 2 * g.R;
+#pragma unroll 1
+      for (int w = 0; w < 2; ++w) {
+        const T* win = static_cast<const T*>(w == 0 ? c.kwin : c.vwin) + d;
+        T* to = w == 0 ? kout : vout + (row0 + p) * (int64_t)values.stride;
+        const uint64_t stride = 4 * (w == 0 ? keys.stride : values.stride);
+        const uint32_t vec = w == 0 ? keys.vec : values.vec;
+        const int packed = w == 0 ? kend : vend;
+        constexpr int kAtOnce = 16 / sizeof(T);  // what registers allow
+        uint4 raw[kAtOnce][sizeof(T) / 2];
+#pragma unroll 1
+        for (int tau0 = (int)p; tau0 < (int)kPagedBlock; tau0 += 4 * kAtOnce, to += kAtOnce * stride) {
+#pragma unroll
+          for (int i = 0; i < kAtOnce; ++i) {
+            const int tau = tau0 + 4 * i;
+            const T* row = win + (window + ring_row(g, base + tau)) * g.DW;
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(T) / 2; ++k)
+              raw[i][k] = tau >= packed && tau < nend ? reinterpret_cast<const uint4*>(row)[k] : make_uint4(0, 0, 0, 0);
+          }
+#pragma unroll
+          for (int i = 0; i < kAtOnce; ++i) {
+            const int tau = tau0 + 4 * i;
+            if (tau >= lo && tau < hi && tau >= packed)
+              copy8(reinterpret_cast<const T*>(raw[i]), to + i * stride, VEC || vec != 0, VEC ? 8 : D - d);
+          }
+        }
+      }
     }
   }
 }
@@ -567,7 +599,10 @@ hipError_t read_typed(const PagedView& c, const PagedBatch& b, const int32_t* fi
   const PagedGeometry& g = c.geo;
   const uint64_t items = ((uint64_t)b.max_rows + 2 * (kPagedBlock - 1)) / kPagedBlock * g.heads;
   const dim3 grid((uint32_t)((items + kThreads / 64 - 1) / (kThreads / 64)), 1, b.sequences);
-  const auto kernel = g.bits == 2 ? k_paged_read<T, 2> : g.bits == 4 ? k_paged_read<T, 4> : k_paged_read<T, 8>;
+  const bool vec = g.G % 8 == 0 && keys.vec != 0 && values.vec != 0;
+  const auto kernel = g.bits == 2 ? vec ? k_paged_read<T, 2, true> : k_paged_read<T, 2, false>
+                      : g.bits == 4 ? vec ? k_paged_read<T, 4, true> : k_paged_read<T, 4, false>
+                                    : vec ? k_paged_read<T, 8, true> : k_paged_read<T, 8, false>;
   hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, c, b, first, keys, values, magic_of(g.S()), magic_of(4 * g.S()));
   return hipGetLastError();
 }
