@@ -50,6 +50,11 @@ __device__ __forceinline__ float max_with(float x) {
   swapped<BY>(x, &a, &b);
   return fmaxf(a, b);
 }
+// The largest of three, NaN if one is (of a row's logits: its weights are then NaN too); fmaxf would first
+// have to quiet each.
+__device__ __forceinline__ float max_of(float a, float b, float c) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
 // Sum over the lanes of a row of 16 that lie N apart (N 4 or 8), in every lane.
 template <int N>
 __device__ __forceinline__ float sum_row(float x) {
@@ -130,21 +135,35 @@ __device__ __forceinline__ const T* row_of(const PagedGeometry& g, const void* w
   return static_cast<const T*>(rows.p) + (uint64_t)(s.row0 + (t - s.n)) * rows.stride + (uint64_t)head * rows.pitch;
 }
 
+// Eight elements as 16-byte pieces and back, by value: through a pointer they would pass through memory.
+template <class T>
+__device__ __forceinline__ typename Row<T>::Frag frag_of(const u32x4* x) {
+  if constexpr (sizeof(T) == 2) {
+    return __builtin_bit_cast(typename Row<T>::Frag, x[0]);
+  } else {
+    return __builtin_bit_cast(f32x8, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+}
+template <class T>
+__device__ __forceinline__ void pieces_of(typename Row<T>::Frag f, u32x4* x) {
+  if constexpr (sizeof(T) == 2) {
+    x[0] = __builtin_bit_cast(u32x4, f);
+  } else {
+    x[0] = __builtin_bit_cast(u32x4, __builtin_shufflevector(f, f, 0, 1, 2, 3));
+    x[1] = __builtin_bit_cast(u32x4, __builtin_shufflevector(f, f, 4, 5, 6, 7));
+  }
+}
 // Elements d .. d + 7 of a row (d a multiple of 8 under DW).
 template <class T>
 __device__ __forceinline__ typename Row<T>::Frag load_frag(const T* p, uint32_t d) {
-  typename Row<T>::Frag f;
-  u32x4* e = reinterpret_cast<u32x4*>(&f);
-  e[0] = reinterpret_cast<const u32x4*>(p + d)[0];
-  if constexpr (sizeof(T) == 4) e[1] = reinterpret_cast<const u32x4*>(p + d)[1];
-  return f;
+  u32x4 x[sizeof(T) / 2];
+  x[0] = reinterpret_cast<const u32x4*>(p + d)[0];
+  if constexpr (sizeof(T) == 4) x[1] = reinterpret_cast<const u32x4*>(p + d)[1];
+  return frag_of<T>(x);
 }
 template <class T>
 __device__ __forceinline__ typename Row<T>::Frag zero_frag() {
-  typename Row<T>::Frag f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = (T)0.f;
-  return f;
+  return typename Row<T>::Frag{};
 }
 // Whether any of the eight is infinite or NaN.
 template <class T>

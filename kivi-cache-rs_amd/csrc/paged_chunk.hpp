@@ -106,10 +106,11 @@ __device__ __forceinline__ int64_t left_of(const PagedAttention& a, int64_t pos)
   return a.window != 0 ? pos - (int64_t)a.window : -1;
 }
 
-// x, of which the compiler does not know that it stays the same from turn to turn of a loop: what a rare
-// path derives from it is computed there and not kept in registers across the loop.
-__device__ __forceinline__ uint32_t anew(uint32_t x) {
-  asm volatile("" : "+v"(x));
+// The lane, read anew where it stands: what is derived from it is computed there and not kept in registers
+// across the loop (nor the lane itself).
+__device__ __forceinline__ uint32_t lane_anew() {
+  uint32_t x;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=&v"(x));
   return x;
 }
 
@@ -139,24 +140,36 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
   const Walk w = walk_of(a, s, tile_row, tile_end, gq, TT);
   const Part part = part_of(w.tiles, splits, plan.least, split);
   if (split >= part.count) return;
+  // positions of the wave's first and last row and of the workgroup's first
+  const int64_t at0 = w.total - s.m, first_pos = at0 + tile_row / gq;
 
   const uint32_t D = g.D, DW = g.DW, ncg = g.ncg;
   const int64_t kq = paged_kq(g, s.n), vq = paged_vq(g, s.n);
-  const uint32_t row = tile_row + wave * 32 + col;
-  const bool live = row < rows;
-  const uint32_t token = (live ? row : rows - 1) / gq, qhead = head * gq + (live ? row : rows - 1) % gq;
-  // positions of the row, of the wave's first and last row and of the workgroup's first
-  const int64_t at0 = w.total - s.m, pos = at0 + token, first_pos = at0 + tile_row / gq;
+  // the lane's row of the KV head (the last one in lanes past it): worked out where it is wanted
+  const auto row_now = [&] {
+    const uint32_t row = tile_row + wave * 32 + lane_anew() % 32;
+    return row < rows ? row : rows - 1;
+  };
   const uint32_t wr0 = tile_row + wave * 32 < rows ? tile_row + wave * 32 : rows - 1, wr1 = wr0 + 31 < rows ? wr0 + 31 : rows - 1;
   const int64_t all_pos = at0 + wr0 / gq, any_pos = at0 + wr1 / gq;
   // tokens up to here are outside the window: of the wave's last row, of the workgroup's
   const int64_t all_left = a.window != 0 ? any_pos - (int64_t)a.window : -1;
   const int64_t last_left = a.window != 0 ? w.hi - 1 - (int64_t)a.window : -1;
+  // Tiles [plain_at, plain_at + plains) of the walk are packed and seen by every row (where their pages are
+  // there): a loop of their own, with nothing else in it. They come first, then the others.
+  uint32_t plain_at = 0, plains = 0;
+  if constexpr (BITS != 0) {
+    const int64_t seen = first_pos + 1 < vq ? first_pos + 1 : vq;
+    const uint32_t from = last_left < 0 ? 0 : (uint32_t)((last_left + TT) / TT), to = seen < 0 ? 0 : (uint32_t)(seen / TT);
+    const uint32_t first = from > w.first_tile ? from : w.first_tile;
+    if (to > first) plain_at = w.head_tiles + (first - w.first_tile), plains = to - first;
+  }
 
   // exp2(scale q k) with a scale above zero (hidden logits are -inf): a sign, or a zero, goes to the queries
   const float sign = a.scale < 0.f ? -1.f : a.scale == 0.f ? 0.f : 1.f, scale = a.scale == 0.f ? 1.f : fabsf(a.scale) * kLog2e;
   Frag q[DP / 16];
   {
+    const uint32_t row = row_now(), token = row / gq, qhead = head * gq + row % gq;
     const T* p = static_cast<const T*>(a.query.p) + (uint64_t)(s.row0 + token) * a.query.stride + (uint64_t)qhead * a.query.pitch;
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
@@ -199,7 +212,8 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
   };
   const auto locate = [&](uint32_t it) {
     Next n;
-    n.t0 = (int64_t)(it < w.head_tiles ? it : w.first_tile + (it - w.head_tiles)) * TT;
+    const uint32_t at = it - plains < plain_at ? it - plains : it;  // of the walk
+    n.t0 = (int64_t)(at < w.head_tiles ? at : w.first_tile + (at - w.head_tiles)) * TT;
     bool all = true;
     n.keys = clamped(kq - n.t0, 0, TT), n.values = clamped(vq - n.t0, 0, TT);
 #pragma unroll
@@ -222,7 +236,7 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
     const uint32_t* rec;
   };
   const auto unit_of = [&](const Next& n, int e) {
-    const uint32_t u = anew(tid) + e * kThreads;
+    const uint32_t u = (wave + e * WAVES) * 64 + lane_anew();
     Unit x;
     x.b = u / (64 * S), x.i = u / 64 % S, x.l = u % 64, x.q = x.l / 16;
     x.rec = x.b == 0 ? n.rec[0] : n.rec[1];
@@ -251,14 +265,13 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
         for (int k = 0; k < 4; ++k) stage[4 * e + k] = p[k];
       }
     } else {
-      const uint32_t me = anew(tid);
+      const uint32_t me = wave * 64 + lane_anew();
 #pragma unroll
       for (int k = 0; k < kKeyRows; ++k) {
         const uint32_t u = me + k * kThreads, tau = u / (DP / 8), d = u % (DP / 8) * 8;
         Frag f = zero_frag<T>();
         if ((int)tau >= n.keys && n.t0 + tau < w.hi && d < DW && u < kKeyPieces) f = load_frag(row_of<T>(g, a.c.kwin, s, head, n.t0 + tau, a.keys), d);
-#pragma unroll
-        for (int i = 0; i < kWide; ++i) stage[k * kWide + i] = reinterpret_cast<const u32x4*>(&f)[i];
+        pieces_of<T>(f, &stage[k * kWide]);
       }
     }
   };
@@ -280,7 +293,7 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
         }
       }
     } else {
-      const uint32_t me = anew(tid);
+      const uint32_t me = wave * 64 + lane_anew();
 #pragma unroll
       for (int k = 0; k < kValueRows; ++k) {
         const uint32_t u = me + k * kThreads, tau = u % (TT / 2) * 2, d = u / (TT / 2) * 8;
@@ -288,8 +301,7 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
         for (int i = 0; i < 2; ++i) {
           Frag f = zero_frag<T>();
           if ((int)tau + i >= n.values && d < DW && n.t0 + tau + i < w.hi) f = load_frag(row_of<T>(g, a.c.vwin, s, head, n.t0 + tau + i, a.values), d);
-#pragma unroll
-          for (int j = 0; j < kWide; ++j) stage[(2 * k + i) * kWide + j] = reinterpret_cast<const u32x4*>(&f)[j];
+          pieces_of<T>(f, &stage[(2 * k + i) * kWide]);
         }
       }
     }
@@ -316,7 +328,7 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
         }
       }
     } else {
-      const uint32_t me = anew(tid);
+      const uint32_t me = wave * 64 + lane_anew();
 #pragma unroll
       for (int k = 0; k < kKeyRows; ++k) {
         const uint32_t u = me + k * kThreads, tau = u / (DP / 8), d = u % (DP / 8) * 8;
@@ -370,7 +382,7 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
         }
       }
     } else {
-      const uint32_t me = anew(tid);
+      const uint32_t me = wave * 64 + lane_anew();
 #pragma unroll
       for (int k = 0; k < kValueRows; ++k) {
         const uint32_t u = me + k * kThreads, tau = u % (TT / 2) * 2, d = u / (TT / 2) * 8;
@@ -378,8 +390,7 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
         Frag f[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-#pragma unroll
-          for (int j = 0; j < kWide; ++j) reinterpret_cast<u32x4*>(&f[i])[j] = stage[(2 * k + i) * kWide + j];
+          f[i] = frag_of<T>(&stage[(2 * k + i) * kWide]);
           if (n.edge && wild<T>(f[i])) {
             atomicOr(&marks[tau / 32], 1u << (tau + i) % 32);
 #pragma unroll
@@ -468,50 +479,283 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
   };
   const auto whole = [](int packed) { return packed == 0 || packed == TT; };
 
-  Next now = locate(part.from);
-  if (part.from < part.to) {
+  // logit += keys . queries; four fragments are read while the four before are multiplied
+  const auto add_logits = [&](f32x16(&logit)[kSub], const T* keys) {
+    Frag f[2][4];
+    constexpr int kAll = DP / 16 * (int)kSub, kGroups = (kAll + 3) / 4;
+    const auto read = [&](int n) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = (4 * n + j) / (int)kSub, sub = (4 * n + j) % (int)kSub;
+        if (4 * n + j < kAll) f[n % 2][j] = *reinterpret_cast<const Frag*>(keys + (32 * sub + col) * kKeyPitch + 16 * i + 8 * half);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    read(0);
+#pragma unroll
+    for (int n = 0; n < kGroups; ++n) {
+      if (n + 1 < kGroups) read(n + 1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int i = (4 * n + j) / (int)kSub, sub = (4 * n + j) % (int)kSub;
+        if (4 * n + j < kAll) logit[sub] = Mma<T>::mul(f[n % 2][j], q[i], logit[sub]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // acc += values^T . weights; two products of two steps of 32 channels at a time (the last of an odd number: of one)
+  const auto add_values = [&](const Frag(&p)[kSub][2], const T* values) {
+    Frag f[2][4];
+    constexpr int kAll = DP / 32 * (int)kSub * 2, kGroups = (kAll + 3) / 4;
+    const auto step = [](int x, int* i, int* sub, int* u) {
+      constexpr int kEven = DP / 64 * 2, kOf = 2 * (int)kSub;  // products of a step
+      const bool two = x < kEven * kOf;
+      *i = two ? x / (2 * kOf) * 2 + x % 2 : kEven;
+      const int y = two ? x % (2 * kOf) / 2 : x - kEven * kOf;
+      *sub = y / 2, *u = y % 2;
+    };
+    const auto read = [&](int n) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        int i, sub, u;
+        step(4 * n + j, &i, &sub, &u);
+        if (4 * n + j < kAll) f[n % 2][j] = *reinterpret_cast<const Frag*>(values + (32 * i + col) * kValuePitch + 32 * sub + 16 * u + 8 * half);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    read(0);
+#pragma unroll
+    for (int n = 0; n < kGroups; ++n) {
+      if (n + 1 < kGroups) read(n + 1);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        int i, sub, u;
+        step(4 * n + j, &i, &sub, &u);
+        if (4 * n + j < kAll) acc[i] = Mma<T>::mul(f[n % 2][j], p[sub][u], acc[i]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  // Softmax: the running maximum and sum, what is summed so far rescaled, logits to weights.
+  const auto weigh = [&](const f32x16(&logit)[kSub], Frag(&p)[kSub][2]) {
+    float higher = top;
+#pragma unroll
+    for (uint32_t sub = 0; sub < kSub; ++sub)
+#pragma unroll
+      for (uint32_t i = 0; i < 16; i += 2) higher = max_of(higher, logit[sub][i], logit[sub][i + 1]);
+    higher = max_with<32>(higher);
+    const float base = higher == -INFINITY ? 0.f : higher * scale;  // a row that has seen nothing yet
+    // always: a branch round it has the sums in two sets of registers where it joins
+    const float keep = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(fmaf(top, scale, -base));
+    sum *= keep;
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) acc[i] *= keep;
+    top = higher;
+#pragma unroll
+    for (uint32_t sub = 0; sub < kSub; ++sub) {
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) {
+        const float x = __builtin_amdgcn_exp2f(fmaf(logit[sub][i], scale, -base));
+        sum += x;
+        // accumulator rows 8 b + 4 half + j: product u takes b = u and b = u + 2
+        p[sub][i / 4 % 2][i % 4 + (i >= 8 ? 4 : 0)] = (T)x;
+      }
+    }
+  };
+
+  // ---- plain tiles. A wave's units lie in one block each, so all but the lane's place in it is uniform. What
+  // the next tile is made of is fetched a tile ahead, its pages a tile before that.
+  if constexpr (BITS != 0) {
+    const uint32_t to = part.to < plains ? part.to : plains;
+    struct {
+      u32x4 pairs[kEach][4];
+      uint32_t words[kEach][kWords];
+    } keys, values;
+    const auto tile_of = [&](uint32_t it) {  // in the sequence
+      const uint32_t at = plain_at + it;
+      return at < w.head_tiles ? at : w.first_tile + (at - w.head_tiles);
+    };
+    const auto look_up = [&](uint32_t it) {  // lane i: page of block i
+      const uint32_t page = quotient(tile_of(it < to ? it : to - 1) * kSub + lane % kSub, g.page_blocks, g.page_magic);
+      return page < a.b.per_sequence ? s.table[page] : -1;
+    };
+    const auto missing = [&](int32_t pages) {  // bit i: block i has no page
+      uint32_t bits = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < kSub; ++i) bits |= (uint32_t)__builtin_amdgcn_readlane(pages, i) < g.pages ? 0u : 1u << i;
+      return bits;
+    };
+    // record and place in the page of the wave's unit e (no page: the pool's first)
+    const auto place_of = [&](uint32_t it, int32_t pages, int e, const uint32_t** rec, uint32_t* inner, uint32_t* i) {
+      const uint32_t unit = wave + e * WAVES, b = unit / S, block = tile_of(it) * kSub + b;
+      *i = unit % S;
+      *inner = block - quotient(block, g.page_blocks, g.page_magic) * g.page_blocks;
+      const uint32_t page = __builtin_amdgcn_readlane(pages, b);
+      *rec = a.c.pages + ((uint64_t)(page < g.pages ? page : 0) * g.heads + head) * g.record_words;
+    };
+    const auto mine = [&](int e) { return kSub * S % WAVES == 0 || wave + e * WAVES < kSub * S; };
+    const auto at = [](const uint32_t* p, uint32_t words) { return reinterpret_cast<const char*>(p) + words * 4; };
+    const auto fetch_plain_keys = [&](uint32_t it, int32_t pages) {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        if (!mine(e)) continue;
+        const uint32_t* rec;
+        uint32_t inner, i;
+        place_of(it, pages, e, &rec, &inner, &i);
+        const char* from = at(rec + inner * (DP * BITS), lane * LW);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if constexpr (BITS == 8) {
+            keys.words[e][2 * h] = reinterpret_cast<const uint32_t*>(from)[2 * (h * S + i)];
+            keys.words[e][2 * h + 1] = reinterpret_cast<const uint32_t*>(from)[2 * (h * S + i) + 1];
+          } else {
+            keys.words[e][h] = reinterpret_cast<const uint32_t*>(from)[BITS == 2 ? (h * S + i) >> 1 : h * S + i];
+          }
+        }
+        const char* p = at(rec + g.kparams_at + (quotient(inner * 32, g.G, g.group_magic) * DP + 8 * i) * 2, lane / 16 * (16 * S));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) keys.pairs[e][k] = reinterpret_cast<const u32x4*>(p)[k];
+      }
+    };
+    const auto fetch_plain_values = [&](uint32_t it, int32_t pages) {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        if (!mine(e)) continue;
+        const uint32_t* rec;
+        uint32_t inner, i;
+        place_of(it, pages, e, &rec, &inner, &i);
+        const char* from = at(rec + g.vcodes_at + inner * (DP * BITS) + BITS / 2 * i, lane * LW);
+#pragma unroll
+        for (int k = 0; k < BITS / 2; ++k) values.words[e][k] = reinterpret_cast<const uint32_t*>(from)[k];
+        const uint32_t* pairs = rec + g.vparams_at + (inner * 32 * ncg + quotient(32 * i, g.G, g.group_magic)) * 2;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t t = k / 2 * 16 + k % 2 * 2;
+          const uint2 y = *reinterpret_cast<const uint2*>(at(pairs + t * ncg * 2, lane / 16 * ncg * 8));
+          const uint2 z = *reinterpret_cast<const uint2*>(at(pairs + (t + 1) * ncg * 2, lane / 16 * ncg * 8));
+          values.pairs[e][k] = u32x4{y.x, y.y, z.x, z.y};
+        }
+      }
+    };
+    const auto decode_by = [](const u32x4(&pairs)[4], float(&x)[8]) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = fmaf(x[j], __uint_as_float(pairs[j / 2][j % 2 * 2]), __uint_as_float(pairs[j / 2][j % 2 * 2 + 1]));
+    };
+    const auto put_plain_keys = [&](T* kt) {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        if (!mine(e)) continue;
+        const uint32_t unit = wave + e * WAVES, b = unit / S, i = unit % S;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x[8];
+          codes_to<BITS>(keys.words[e] + (BITS == 8 ? 2 * h : h), BITS == 2 ? (h * S + i) & 1 : 0, x);
+          decode_by(keys.pairs[e], x);
+          put_terms<T, KT>(x, kt + (32 * b + 16 * h + lane % 16) * kKeyPitch + 8 * S * (lane / 16) + 8 * i, Tile::kKeys);
+        }
+      }
+    };
+    const auto put_plain_values = [&](T* vt, uint32_t gone) {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        if (!mine(e)) continue;
+        const uint32_t unit = wave + e * WAVES, b = unit / S, i = unit % S;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x[8];
+          codes_to<BITS>(values.words[e] + (BITS == 8 ? 2 * h : BITS == 4 ? h : 0), BITS == 2 ? h : 0, x);
+          decode_by(values.pairs[e], x);
+          if (gone >> b & 1) {  // no weight of zero keeps an infinity out
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = 0.f;
+          }
+          put_terms<T, VT>(x, vt + (32 * i + 16 * h + lane % 16) * kValuePitch + 32 * b + 8 * (lane / 16), Tile::kValues);
+        }
+      }
+    };
+    if (part.from < to) {
+      int32_t pages = look_up(part.from), pages_next = look_up(part.from + 1);
+      uint32_t gone = missing(pages), gone_next = missing(pages_next);
+      fetch_plain_keys(part.from, pages);
+      fetch_plain_values(part.from, pages);
+      put_plain_keys(tiles);
+      put_plain_values(tiles + KT * Tile::kKeys, gone);
+      fetch_plain_keys(part.from + 1 < to ? part.from + 1 : part.from, pages_next);
+      fetch_plain_values(part.from + 1 < to ? part.from + 1 : part.from, pages_next);
+      pages = look_up(part.from + 2);
+      T* kt = tiles;
+      T* other = tiles + Tile::kElements;
+#pragma unroll 1
+      for (uint32_t it = part.from; it < to; ++it) {
+        __syncthreads();  // this tile is filled, the other one read
+        pages_next = look_up(it + 3);
+        const uint32_t then = it + 2 < to ? it + 2 : to - 1;  // fetched again behind the end, and dropped
+        __builtin_amdgcn_sched_barrier(0);
+        f32x16 logit[kSub];
+#pragma unroll
+        for (uint32_t sub = 0; sub < kSub; ++sub) logit[sub] = f32x16{0.f};
+        add_logits(logit, kt);
+        if constexpr (KT == 2) add_logits(logit, kt + Tile::kKeys);
+        if (gone != 0) {
+#pragma unroll
+          for (uint32_t sub = 0; sub < kSub; ++sub)
+            if (gone >> sub & 1) {
+#pragma unroll
+              for (uint32_t i = 0; i < 16; ++i) logit[sub][i] = -INFINITY;
+            }
+        }
+        Frag p[kSub][2];
+        weigh(logit, p);
+        __builtin_amdgcn_sched_barrier(0);
+        put_plain_keys(other);
+        __builtin_amdgcn_sched_barrier(0);
+        gone = gone_next, gone_next = missing(pages);
+        fetch_plain_keys(then, pages);
+        __builtin_amdgcn_sched_barrier(0);
+        add_values(p, kt + KT * Tile::kKeys);
+        if constexpr (VT == 2) add_values(p, kt + KT * Tile::kKeys + Tile::kValues);
+        put_plain_values(other + KT * Tile::kKeys, gone);  // of the next tile by now
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_plain_values(then, pages);
+        pages = pages_next;
+        T* const swap = kt;
+        kt = other, other = swap;
+      }
+      __syncthreads();
+    }
+  }
+
+  // ---- the other tiles
+  const uint32_t from = part.from > plains ? part.from : plains;
+  Next now = locate(from);
+  if (from < part.to) {
     if constexpr (BITS == 0)
-      fill_any(now, tiles, bad[part.from % 3]);
+      fill_any(now, tiles, bad[from % 3]);
     else
-      fill_both(now, true, true, tiles, bad[part.from % 3]);
+      fill_both(now, true, true, tiles, bad[from % 3]);
   }
 #pragma unroll 1
-  for (uint32_t it = part.from; it < part.to; ++it) {
+  for (uint32_t it = from; it < part.to; ++it) {
     __syncthreads();  // this tile is filled, the other one read
     if (tid < 2) bad[(it + 2) % 3][tid] = 0;
     const bool more = it + 1 < part.to;
     const Next next = locate(more ? it + 1 : it);
     if (BITS != 0 && more && whole(next.keys)) fetch_keys(next, next.keys > 0);
-    const T* kt = tiles + (it - part.from) % 2 * Tile::kElements;
+    const T* kt = tiles + (it - from) % 2 * Tile::kElements;
     const T* vt = kt + KT * Tile::kKeys;
-    T* next_kt = tiles + (it + 1 - part.from) % 2 * Tile::kElements;
+    T* next_kt = tiles + (it + 1 - from) % 2 * Tile::kElements;
     const int64_t t0 = now.t0;
     const bool two_keys = BITS == 0 || now.keys > 0, two_values = BITS == 0 || now.values > 0;  // both terms
     // phases one after the other: interleaved, they want more registers than there are
     __builtin_amdgcn_sched_barrier(0);
     f32x16 logit[kSub];
 #pragma unroll
-    for (uint32_t sub = 0; sub < kSub; ++sub) {
-      logit[sub] = f32x16{0.f};
-#pragma unroll
-      for (int i = 0; i < DP / 16; ++i) {
-        logit[sub] = Mma<T>::mul(*reinterpret_cast<const Frag*>(kt + (32 * sub + col) * kKeyPitch + 16 * i + 8 * half), q[i], logit[sub]);
-        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    if (KT == 2 && two_keys) {
-#pragma unroll
-      for (uint32_t sub = 0; sub < kSub; ++sub) {
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-          logit[sub] = Mma<T>::mul(*reinterpret_cast<const Frag*>(kt + Tile::kKeys + (32 * sub + col) * kKeyPitch + 16 * i + 8 * half), q[i],
-                                   logit[sub]);
-          if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-        }
-      }
-    }
+    for (uint32_t sub = 0; sub < kSub; ++sub) logit[sub] = f32x16{0.f};
+    add_logits(logit, kt);
+    if (KT == 2 && two_keys) add_logits(logit, kt + Tile::kKeys);
     if (now.edge && !(t0 + TT - 1 <= all_pos && t0 > all_left && t0 >= kq)) {
-      const int mine = (int)anew(4 * half);
+      const int mine = (int)(lane_anew() / 32 * 4);
+      const int64_t pos = at0 + row_now() / gq;
 #pragma unroll
       for (uint32_t sub = 0; sub < kSub; ++sub) {
         // counted from the sub-tile's first token
@@ -526,61 +770,16 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
         }
       }
     }
-    float peak = logit[0][0];
-#pragma unroll
-    for (uint32_t sub = 0; sub < kSub; ++sub)
-#pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) peak = fmaxf(peak, logit[sub][i]);
-    peak = fmaxf(peak, __shfl_xor(peak, 32));
-    const float higher = fmaxf(top, peak);
-    const float base = higher == -INFINITY ? 0.f : higher * scale;  // a row that has seen nothing yet
-    if (__any(higher != top)) {
-      const float keep = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(fmaf(top, scale, -base));
-      sum *= keep;
-#pragma unroll
-      for (int i = 0; i < DP / 32; ++i) acc[i] *= keep;
-    }
-    top = higher;
     Frag p[kSub][2];
-#pragma unroll
-    for (uint32_t sub = 0; sub < kSub; ++sub) {
-#pragma unroll
-      for (uint32_t i = 0; i < 16; ++i) {
-        const float x = __builtin_amdgcn_exp2f(fmaf(logit[sub][i], scale, -base));
-        sum += x;
-        // accumulator rows 8 b + 4 half + j: product u takes b = u and b = u + 2
-        p[sub][i / 4 % 2][i % 4 + (i >= 8 ? 4 : 0)] = (T)x;
-      }
-    }
+    weigh(logit, p);
     __builtin_amdgcn_sched_barrier(0);
     if (BITS != 0 && more) {
       if (whole(next.keys)) put_keys(next, next.keys > 0, next_kt);
       if (whole(next.values)) fetch_values(next, next.values > 0);
     }
     __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < DP / 32; ++i) {
-#pragma unroll
-      for (uint32_t sub = 0; sub < kSub; ++sub)
-#pragma unroll
-        for (uint32_t u = 0; u < 2; ++u)
-          acc[i] = Mma<T>::mul(*reinterpret_cast<const Frag*>(vt + (32 * i + col) * kValuePitch + 32 * sub + 16 * u + 8 * half), p[sub][u],
-                               acc[i]);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    if (VT == 2 && two_values) {
-#pragma unroll
-      for (int i = 0; i < DP / 32; ++i) {
-#pragma unroll
-        for (uint32_t sub = 0; sub < kSub; ++sub)
-#pragma unroll
-          for (uint32_t u = 0; u < 2; ++u)
-            acc[i] = Mma<T>::mul(
-                *reinterpret_cast<const Frag*>(vt + Tile::kValues + (32 * i + col) * kValuePitch + 32 * sub + 16 * u + 8 * half), p[sub][u],
-                acc[i]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
+    add_values(p, vt);
+    if (VT == 2 && two_values) add_values(p, vt + Tile::kValues);
     if (now.edge && (bad[it % 3][0] | bad[it % 3][1]) != 0) {
 #pragma unroll
       for (uint32_t sub = 0; sub < kSub; ++sub) {
@@ -589,7 +788,7 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
           const int64_t t = t0 + 32 * sub + tau;
           wave_fence();
 #pragma unroll 1
-          for (uint32_t d = anew(lane); d < DP; d += 64) {
+          for (uint32_t d = lane_anew(); d < DP; d += 64) {
             const float x = d < D ? value_of<T>(a, s, now.rec[sub], head, t, vq, d) : 0.f;
             bad_row[wave][d] = fabsf(x) <= kLargest ? 0.f : x;
           }
@@ -599,8 +798,9 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
           for (uint32_t i = 0; i < 16; ++i)
             if (i == tau / 8 * 4 + tau % 4) weight = (float)p[sub][i / 4 % 2][i % 4 + (i >= 8 ? 4 : 0)];
           weight = __shfl(weight, (int)(tau % 8 / 4 * 32 + col));
+          const int64_t pos = at0 + row_now() / gq;
           const bool seen = t <= pos && (t > left_of(a, pos) || t < (int64_t)a.sinks);
-          const uint32_t mine = anew(4 * half);
+          const uint32_t mine = lane_anew() / 32 * 4;
 #pragma unroll
           for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -621,9 +821,10 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
     now = next;
   }
 
-  sum += __shfl_xor(sum, 32);
-  if (!live) return;
+  sum = sum_with<32>(sum);
+  if (tile_row + wave * 32 + lane_anew() % 32 >= rows) return;
   top *= scale;
+  const uint32_t row = row_now(), token = row / gq, qhead = head * gq + row % gq;
   const uint64_t place = (uint64_t)(s.row0 + token) * a.qh + qhead;
   if (part.count == 1) {
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
