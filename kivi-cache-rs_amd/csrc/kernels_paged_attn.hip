@@ -97,21 +97,26 @@ Plan plan_of(const PagedGeometry& g, const PagedBatch& b, uint32_t qh, uint64_t 
   p.chunks = rows > p.chunk.over;
   p.chunk.tile_rows = paged_chunk_rows(g);
   p.chunk.tile = paged_chunk_tokens(g);
-  p.chunk.least = 4;
+  p.chunk.least = 1;
   const uint64_t groups = std::max<uint64_t>(1, (uint64_t)b.rows * gq / p.chunk.tile_rows) * g.heads;  // about
-  // one workgroup fills a compute unit: the fewest splits whose last round wastes little
-  uint64_t want = 1;
-  double best = 1e30;
-  for (uint64_t n = 1; n <= 64; ++n) {
-    const double rounds = (double)((groups * n + kComputeUnits - 1) / kComputeUnits) / (double)n;
-    if (rounds < 0.85 * best) best = rounds, want = n;
-  }
+  // One workgroup fills a compute unit: rounds of workgroups times the tiles of each (and two for its start and
+  // end), and what a join costs, in tiles of about 3.5 us: its launch, partial sums written and read. Two sequences of 6000 rows
+  // (375 groups) over 18 tiles: 1 split 126 us, 2 splits 181.
   const auto chunk_splits = [&](uint64_t n) {
-    return (uint32_t)std::max<uint64_t>(1, std::min(want, (n + p.chunk.tile - 1) / p.chunk.tile / p.chunk.least));
+    const uint64_t tiles = std::max<uint64_t>(1, (n + p.chunk.tile - 1) / p.chunk.tile);
+    uint64_t best = 1, least_cost = ~(uint64_t)0;
+    for (uint64_t k = 1; k <= std::max<uint64_t>(1, std::min<uint64_t>(64, tiles / 4)); ++k) {
+      const uint64_t rounds = (groups * k + kComputeUnits - 1) / kComputeUnits;
+      const uint64_t cost = rounds * ((tiles + k - 1) / k + 2) + (k == 1 ? 0 : 2 + k * groups * g.DP / 6400);
+      if (cost < least_cost) least_cost = cost, best = k;
+    }
+    return (uint32_t)best;
   };
-  p.chunk.splits = chunk_splits(tokens);
+  const uint32_t most_chunk_splits = chunk_splits(all);
+  const uint64_t walked = window == 0 ? all : std::min(all, window + std::min(sinks, all) + p.chunk.tile_rows / gq + 3 * p.chunk.tile);
+  p.chunk.splits = std::min(chunk_splits(walked), most_chunk_splits);
   p.chunk_at = p.floats;
-  if (p.chunks && chunk_splits(all) > 1) p.floats += (size_t)chunk_splits(all) * (size_t)b.rows * qh * (g.DP + 2);
+  if (p.chunks && most_chunk_splits > 1) p.floats += (size_t)most_chunk_splits * (size_t)b.rows * qh * (g.DP + 2);
   return p;
 }
 

@@ -155,8 +155,13 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
   // tokens up to here are outside the window: of the wave's last row, of the workgroup's
   const int64_t all_left = a.window != 0 ? any_pos - (int64_t)a.window : -1;
   const int64_t last_left = a.window != 0 ? w.hi - 1 - (int64_t)a.window : -1;
-  // Tiles [plain_at, plain_at + plains) of the walk are packed and seen by every row (where their pages are
-  // there): a loop of their own, with nothing else in it. They come first, then the others.
+  // Three kinds of tiles, each with a loop of its own, one after the other: [plain_at, plain_at + plains) of the
+  // walk are packed and seen by every row (where their pages are there); from dense_at on all tokens are rows;
+  // and the others.
+  uint32_t dense_at = (uint32_t)((kq + TT - 1) / TT);
+  if (dense_at >= w.head_tiles) dense_at = w.head_tiles + (dense_at > w.first_tile ? dense_at - w.first_tile : 0);
+  if (dense_at > w.tiles) dense_at = w.tiles;
+  const uint32_t denses = w.tiles - dense_at;
   uint32_t plain_at = 0, plains = 0;
   if constexpr (BITS != 0) {
     const int64_t seen = first_pos + 1 < vq ? first_pos + 1 : vq;
@@ -212,7 +217,7 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
   };
   const auto locate = [&](uint32_t it) {
     Next n;
-    const uint32_t at = it - plains < plain_at ? it - plains : it;  // of the walk
+    const uint32_t at = it - plains - denses < plain_at ? it - plains - denses : it - denses;  // of the walk
     n.t0 = (int64_t)(at < w.head_tiles ? at : w.first_tile + (at - w.head_tiles)) * TT;
     bool all = true;
     n.keys = clamped(kq - n.t0, 0, TT), n.values = clamped(vq - n.t0, 0, TT);
@@ -243,6 +248,84 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
     x.inner = x.b == 0 ? n.inner[0] : n.inner[1];
     return x;
   };
+  // Place of token tau in a row of values. Values that are not finite are left out of a tile that some row
+  // does not see whole (a weight of zero would not keep them from it) and marked.
+  const auto slot = [](uint32_t tau) { return tau / 32 * 32 + tau % 16 / 4 * 8 + tau % 32 / 16 * 4 + tau % 4; };
+  // Rows of a tile from token `from` of it on: 8-channel pieces.
+  const auto fetch_key_rows = [&](u32x4(&stage)[kMost], int64_t t0, int from) {
+    const uint32_t me = wave * 64 + lane_anew();
+#pragma unroll
+    for (int k = 0; k < kKeyRows; ++k) {
+      const uint32_t u = me + k * kThreads, tau = u / (DP / 8), d = u % (DP / 8) * 8;
+      Frag f = zero_frag<T>();
+      if ((int)tau >= from && t0 + tau < w.hi && d < DW && u < kKeyPieces) f = load_frag(row_of<T>(g, a.c.kwin, s, head, t0 + tau, a.keys), d);
+      pieces_of<T>(f, &stage[k * kWide]);
+    }
+  };
+  const auto fetch_value_rows = [&](u32x4(&stage)[kMost], int64_t t0, int from) {
+    const uint32_t me = wave * 64 + lane_anew();
+#pragma unroll
+    for (int k = 0; k < kValueRows; ++k) {
+      const uint32_t u = me + k * kThreads, tau = u % (TT / 2) * 2, d = u / (TT / 2) * 8;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        Frag f = zero_frag<T>();
+        if ((int)tau + i >= from && d < DW && t0 + tau + i < w.hi) f = load_frag(row_of<T>(g, a.c.vwin, s, head, t0 + tau + i, a.values), d);
+        pieces_of<T>(f, &stage[(2 * k + i) * kWide]);
+      }
+    }
+  };
+  const auto put_key_rows = [&](const u32x4(&stage)[kMost], int from, T* kt) {
+    const uint32_t me = wave * 64 + lane_anew();
+#pragma unroll
+    for (int k = 0; k < kKeyRows; ++k) {
+      const uint32_t u = me + k * kThreads, tau = u / (DP / 8), d = u % (DP / 8) * 8;
+      if ((int)tau < from || (kKeyPieces % kThreads != 0 && u >= kKeyPieces)) continue;
+#pragma unroll
+      for (int i = 0; i < kWide; ++i) {
+        reinterpret_cast<u32x4*>(kt + tau * kKeyPitch + d)[i] = stage[k * kWide + i];
+        if (KT == 2 && from > 0) reinterpret_cast<u32x4*>(kt + Tile::kKeys + tau * kKeyPitch + d)[i] = u32x4{0, 0, 0, 0};
+      }
+    }
+  };
+  const auto put_value_rows = [&](const u32x4(&stage)[kMost], int from, bool edge, T* vt, uint32_t* marks) {
+    const uint32_t me = wave * 64 + lane_anew();
+#pragma unroll
+    for (int k = 0; k < kValueRows; ++k) {
+      const uint32_t u = me + k * kThreads, tau = u % (TT / 2) * 2, d = u / (TT / 2) * 8;
+      if (kValuePieces % kThreads != 0 && u >= kValuePieces) continue;
+      Frag f[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f[i] = frag_of<T>(&stage[(2 * k + i) * kWide]);
+        if (edge && wild<T>(f[i])) {
+          atomicOr(&marks[tau / 32], 1u << (tau + i) % 32);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) f[i][j] = fabsf((float)f[i][j]) <= kLargest ? f[i][j] : (T)0.f;
+        }
+      }
+      T* to = vt + d * kValuePitch + slot(tau);
+      if (from == 0) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          struct alignas(2 * sizeof(T)) Two {
+            T x, y;
+          };
+          *reinterpret_cast<Two*>(to + j * kValuePitch) = Two{f[0][j], f[1][j]};
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if ((int)tau + i < from) continue;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            to[j * kValuePitch + i] = f[i][j];
+            if constexpr (VT == 2) to[Tile::kValues + j * kValuePitch + i] = (T)0.f;
+          }
+        }
+      }
+    }
+  };
   // `packed`: the packed part of tile n, else its rows; only a tile that has both is filled in two passes
   const auto fetch_keys = [&](const Next& n, bool packed) {
     if (packed) {
@@ -265,14 +348,7 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
         for (int k = 0; k < 4; ++k) stage[4 * e + k] = p[k];
       }
     } else {
-      const uint32_t me = wave * 64 + lane_anew();
-#pragma unroll
-      for (int k = 0; k < kKeyRows; ++k) {
-        const uint32_t u = me + k * kThreads, tau = u / (DP / 8), d = u % (DP / 8) * 8;
-        Frag f = zero_frag<T>();
-        if ((int)tau >= n.keys && n.t0 + tau < w.hi && d < DW && u < kKeyPieces) f = load_frag(row_of<T>(g, a.c.kwin, s, head, n.t0 + tau, a.keys), d);
-        pieces_of<T>(f, &stage[k * kWide]);
-      }
+      fetch_key_rows(stage, n.t0, n.keys);
     }
   };
   const auto fetch_values = [&](const Next& n, bool packed) {
@@ -293,17 +369,7 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
         }
       }
     } else {
-      const uint32_t me = wave * 64 + lane_anew();
-#pragma unroll
-      for (int k = 0; k < kValueRows; ++k) {
-        const uint32_t u = me + k * kThreads, tau = u % (TT / 2) * 2, d = u / (TT / 2) * 8;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          Frag f = zero_frag<T>();
-          if ((int)tau + i >= n.values && d < DW && n.t0 + tau + i < w.hi) f = load_frag(row_of<T>(g, a.c.vwin, s, head, n.t0 + tau + i, a.values), d);
-          pieces_of<T>(f, &stage[(2 * k + i) * kWide]);
-        }
-      }
+      fetch_value_rows(stage, n.t0, n.values);
     }
   };
   // x[j] = code * scale + zero with the pairs of unit e
@@ -328,22 +394,9 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
         }
       }
     } else {
-      const uint32_t me = wave * 64 + lane_anew();
-#pragma unroll
-      for (int k = 0; k < kKeyRows; ++k) {
-        const uint32_t u = me + k * kThreads, tau = u / (DP / 8), d = u % (DP / 8) * 8;
-        if ((int)tau < n.keys || (kKeyPieces % kThreads != 0 && u >= kKeyPieces)) continue;
-#pragma unroll
-        for (int i = 0; i < kWide; ++i) {
-          reinterpret_cast<u32x4*>(kt + tau * kKeyPitch + d)[i] = stage[k * kWide + i];
-          if (KT == 2 && n.keys > 0) reinterpret_cast<u32x4*>(kt + Tile::kKeys + tau * kKeyPitch + d)[i] = u32x4{0, 0, 0, 0};
-        }
-      }
+      put_key_rows(stage, n.keys, kt);
     }
   };
-  // Place of token tau in a row of values. Values that are not finite are left out of a tile that some row
-  // does not see whole (a weight of zero would not keep them from it) and marked.
-  const auto slot = [](uint32_t tau) { return tau / 32 * 32 + tau % 16 / 4 * 8 + tau % 32 / 16 * 4 + tau % 4; };
   const auto put_values = [&](const Next& n, bool packed, T* vt, uint32_t* marks) {
     if (packed) {
 #pragma unroll
@@ -382,42 +435,7 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
         }
       }
     } else {
-      const uint32_t me = wave * 64 + lane_anew();
-#pragma unroll
-      for (int k = 0; k < kValueRows; ++k) {
-        const uint32_t u = me + k * kThreads, tau = u % (TT / 2) * 2, d = u / (TT / 2) * 8;
-        if (kValuePieces % kThreads != 0 && u >= kValuePieces) continue;
-        Frag f[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          f[i] = frag_of<T>(&stage[(2 * k + i) * kWide]);
-          if (n.edge && wild<T>(f[i])) {
-            atomicOr(&marks[tau / 32], 1u << (tau + i) % 32);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) f[i][j] = fabsf((float)f[i][j]) <= kLargest ? f[i][j] : (T)0.f;
-          }
-        }
-        T* to = vt + d * kValuePitch + slot(tau);
-        if (n.values == 0) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            struct alignas(2 * sizeof(T)) Two {
-              T x, y;
-            };
-            *reinterpret_cast<Two*>(to + j * kValuePitch) = Two{f[0][j], f[1][j]};
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if ((int)tau + i < n.values) continue;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              to[j * kValuePitch + i] = f[i][j];
-              if constexpr (VT == 2) to[Tile::kValues + j * kValuePitch + i] = (T)0.f;
-            }
-          }
-        }
-      }
+      put_value_rows(stage, n.values, n.edge, vt, marks);
     }
   };
   // A layout that the units do not know (groups of no multiple of 32, other head widths): element by element.
@@ -559,6 +577,55 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
         sum += x;
         // accumulator rows 8 b + 4 half + j: product u takes b = u and b = u + 2
         p[sub][i / 4 % 2][i % 4 + (i >= 8 ? 4 : 0)] = (T)x;
+      }
+    }
+  };
+
+  // Logits of what a row does not see (held: whether the blocks' pages are there) become -inf.
+  const auto hide = [&](f32x16(&logit)[kSub], int64_t t0, bool held0, bool held1) {
+    const int mine = (int)(lane_anew() / 32 * 4);
+    const int64_t pos = at0 + row_now() / gq;
+#pragma unroll
+    for (uint32_t sub = 0; sub < kSub; ++sub) {
+      // counted from the sub-tile's first token
+      const int64_t from = t0 + 32 * sub;
+      const int see_to = clamped(pos - from, -1, 31), see_from = clamped(left_of(a, pos) - from, -1, 31);
+      const int sinks = clamped((int64_t)a.sinks - from, 0, 32), held = (sub == 0 ? held0 : held1) ? 0 : clamped(kq - from, 0, 32);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int tau = 8 * (i / 4) + mine + i % 4;
+        const bool seen = tau <= see_to && (tau > see_from || tau < sinks) && tau >= held;
+        logit[sub][i] = seen ? logit[sub][i] : -INFINITY;
+      }
+    }
+  };
+  // Values that were left out of a tile, for the rows that see them.
+  const auto add_bad = [&](const Frag(&p)[kSub][2], const uint32_t* marks, int64_t t0, const uint32_t* rec0, const uint32_t* rec1) {
+#pragma unroll
+    for (uint32_t sub = 0; sub < kSub; ++sub) {
+      for (uint32_t rest = marks[sub]; rest != 0; rest &= rest - 1) {
+        const uint32_t tau = __ffs(rest) - 1;
+        const int64_t t = t0 + 32 * sub + tau;
+        wave_fence();
+#pragma unroll 1
+        for (uint32_t d = lane_anew(); d < DP; d += 64) {
+          const float x = d < D ? value_of<T>(a, s, sub == 0 ? rec0 : rec1, head, t, vq, d) : 0.f;
+          bad_row[wave][d] = fabsf(x) <= kLargest ? 0.f : x;
+        }
+        wave_fence();
+        float weight = 0.f;
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i)
+          if (i == tau / 8 * 4 + tau % 4) weight = (float)p[sub][i / 4 % 2][i % 4 + (i >= 8 ? 4 : 0)];
+        weight = __shfl(weight, (int)(tau % 8 / 4 * 32 + col));
+        const int64_t pos = at0 + row_now() / gq;
+        const bool seen = t <= pos && (t > left_of(a, pos) || t < (int64_t)a.sinks);
+        const uint32_t mine = lane_anew() / 32 * 4;
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+          for (uint32_t e = 0; e < 16; ++e)
+            if (seen) acc[i][e] += weight * bad_row[wave][32 * i + 8 * (e / 4) + mine + e % 4];
       }
     }
   };
@@ -725,8 +792,61 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
     }
   }
 
+  // ---- tiles of rows, fetched a tile ahead
+  {
+    const uint32_t first = part.from > plains ? part.from : plains, to = part.to < plains + denses ? part.to : plains + denses;
+    const auto start_of = [&](uint32_t it) {
+      const uint32_t at = dense_at + (it < to ? it : to - 1) - plains;
+      return (int64_t)(at < w.head_tiles ? at : w.first_tile + (at - w.head_tiles)) * TT;
+    };
+    const auto edge_of = [&](int64_t t0) { return t0 + TT - 1 > first_pos || t0 <= last_left; };
+    u32x4 key_rows[kMost], value_rows[kMost];
+    if (first < to) {
+      int64_t t0 = start_of(first), next = start_of(first + 1);
+      fetch_key_rows(key_rows, t0, 0);
+      fetch_value_rows(value_rows, t0, 0);
+      put_key_rows(key_rows, 0, tiles);
+      put_value_rows(value_rows, 0, edge_of(t0), tiles + KT * Tile::kKeys, bad[first % 3]);
+      fetch_key_rows(key_rows, next, 0);
+      fetch_value_rows(value_rows, next, 0);
+      T* kt = tiles;
+      T* other = tiles + Tile::kElements;
+#pragma unroll 1
+      for (uint32_t it = first; it < to; ++it) {
+        __syncthreads();  // this tile is filled, the other one read
+        if (tid < 2) bad[(it + 2) % 3][tid] = 0;
+        const int64_t then = start_of(it + 2);  // the last one again behind the end, dropped
+        const bool edge = edge_of(t0);
+        __builtin_amdgcn_sched_barrier(0);
+        f32x16 logit[kSub];
+#pragma unroll
+        for (uint32_t sub = 0; sub < kSub; ++sub) logit[sub] = f32x16{0.f};
+        add_logits(logit, kt);
+        if (edge && !(t0 + TT - 1 <= all_pos && t0 > all_left)) hide(logit, t0, true, true);
+        Frag p[kSub][2];
+        weigh(logit, p);
+        __builtin_amdgcn_sched_barrier(0);
+        put_key_rows(key_rows, 0, other);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_key_rows(key_rows, then, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        add_values(p, kt + KT * Tile::kKeys);
+        if (edge && (bad[it % 3][0] | bad[it % 3][1]) != 0) add_bad(p, bad[it % 3], t0, nullptr, nullptr);
+        if (it + 1 < to) put_value_rows(value_rows, 0, edge_of(next), other + KT * Tile::kKeys, bad[(it + 1) % 3]);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch_value_rows(value_rows, then, 0);
+        t0 = next, next = then;
+        T* const swap = kt;
+        kt = other, other = swap;
+      }
+      __syncthreads();
+      if (tid < 6) bad[tid / 2][tid % 2] = 0;
+      __syncthreads();
+    }
+  }
+
   // ---- the other tiles
-  const uint32_t from = part.from > plains ? part.from : plains;
+  const uint32_t from = part.from > plains + denses ? part.from : plains + denses;
   Next now = locate(from);
   if (from < part.to) {
     if constexpr (BITS == 0)
@@ -753,23 +873,7 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
     for (uint32_t sub = 0; sub < kSub; ++sub) logit[sub] = f32x16{0.f};
     add_logits(logit, kt);
     if (KT == 2 && two_keys) add_logits(logit, kt + Tile::kKeys);
-    if (now.edge && !(t0 + TT - 1 <= all_pos && t0 > all_left && t0 >= kq)) {
-      const int mine = (int)(lane_anew() / 32 * 4);
-      const int64_t pos = at0 + row_now() / gq;
-#pragma unroll
-      for (uint32_t sub = 0; sub < kSub; ++sub) {
-        // counted from the sub-tile's first token
-        const int64_t from = t0 + 32 * sub;
-        const int see_to = clamped(pos - from, -1, 31), see_from = clamped(left_of(a, pos) - from, -1, 31);
-        const int sinks = clamped((int64_t)a.sinks - from, 0, 32), held = now.held[sub] ? 0 : clamped(kq - from, 0, 32);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int tau = 8 * (i / 4) + mine + i % 4;
-          const bool seen = tau <= see_to && (tau > see_from || tau < sinks) && tau >= held;
-          logit[sub][i] = seen ? logit[sub][i] : -INFINITY;
-        }
-      }
-    }
+    if (now.edge && !(t0 + TT - 1 <= all_pos && t0 > all_left && t0 >= kq)) hide(logit, t0, now.held[0], now.held[1]);
     Frag p[kSub][2];
     weigh(logit, p);
     __builtin_amdgcn_sched_barrier(0);
@@ -780,35 +884,7 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
     __builtin_amdgcn_sched_barrier(0);
     add_values(p, vt);
     if (VT == 2 && two_values) add_values(p, vt + Tile::kValues);
-    if (now.edge && (bad[it % 3][0] | bad[it % 3][1]) != 0) {
-#pragma unroll
-      for (uint32_t sub = 0; sub < kSub; ++sub) {
-        for (uint32_t rest = bad[it % 3][sub]; rest != 0; rest &= rest - 1) {
-          const uint32_t tau = __ffs(rest) - 1;
-          const int64_t t = t0 + 32 * sub + tau;
-          wave_fence();
-#pragma unroll 1
-          for (uint32_t d = lane_anew(); d < DP; d += 64) {
-            const float x = d < D ? value_of<T>(a, s, now.rec[sub], head, t, vq, d) : 0.f;
-            bad_row[wave][d] = fabsf(x) <= kLargest ? 0.f : x;
-          }
-          wave_fence();
-          float weight = 0.f;
-#pragma unroll
-          for (uint32_t i = 0; i < 16; ++i)
-            if (i == tau / 8 * 4 + tau % 4) weight = (float)p[sub][i / 4 % 2][i % 4 + (i >= 8 ? 4 : 0)];
-          weight = __shfl(weight, (int)(tau % 8 / 4 * 32 + col));
-          const int64_t pos = at0 + row_now() / gq;
-          const bool seen = t <= pos && (t > left_of(a, pos) || t < (int64_t)a.sinks);
-          const uint32_t mine = lane_anew() / 32 * 4;
-#pragma unroll
-          for (int i = 0; i < DP / 32; ++i)
-#pragma unroll
-            for (uint32_t e = 0; e < 16; ++e)
-              if (seen) acc[i][e] += weight * bad_row[wave][32 * i + 8 * (e / 4) + mine + e % 4];
-        }
-      }
-    }
+    if (now.edge && (bad[it % 3][0] | bad[it % 3][1]) != 0) add_bad(p, bad[it % 3], t0, now.rec[0], now.rec[1]);
     if (more) {
       if constexpr (BITS == 0) {
         fill_any(next, next_kt, bad[(it + 1) % 3]);
