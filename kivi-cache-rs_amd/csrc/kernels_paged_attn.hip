@@ -77,8 +77,8 @@ Plan plan_of(const PagedGeometry& g, const PagedBatch& b, uint32_t qh, uint64_t 
       // blocks of a split and the splits of a walk over n tokens, at most `cap`
       const auto cut = [&](uint64_t n, uint64_t cap) {
         const uint64_t blocks = std::max<uint64_t>(1, (n + kPagedBlock - 1) / kPagedBlock);
-        // one to four turns a wave (what surrounds the turns costs about one), more where there are many
-        const uint64_t turns = std::clamp<uint64_t>(blocks * heads * tiles / turn / 1024, 1, 4);
+        // one to eight turns a wave (what surrounds the turns costs about one), more where there are many
+        const uint64_t turns = std::clamp<uint64_t>(blocks * heads * tiles / turn / 1024, 1, 8);
         const uint64_t least = std::max({turns * turn, blocks * heads * tiles / kRowsWorkgroups, (blocks + cap - 1) / cap});
         r.least = (uint32_t)((least + turn - 1) / turn * turn);
         r.splits = (uint32_t)((blocks + r.least - 1) / r.least);

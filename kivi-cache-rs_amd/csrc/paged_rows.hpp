@@ -420,20 +420,23 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
           unseen |= seen ? 0u : 1u << j;
         }
       }
-      weigh(x);
-
-      // ---- output: the values' pairs go to LDS, the next turn's keys are fetched
-#pragma unroll
-      for (int b = 0; b < BLOCKS; ++b)
-#pragma unroll
-        for (int i = 0; i < kValueLoads; ++i) *reinterpret_cast<f32x4*>(vpairs + b * vblock + vput[i]) = vp[b][i];
-      wave_fence();
+      // the next turn's keys are fetched as soon as this one's are done with
+      __builtin_amdgcn_sched_barrier(0);
       at += 4 * BLOCKS;
       if (at < to) {
         locate();
         load_keys();
         look_up(at + 4 * BLOCKS);
       }
+      __builtin_amdgcn_sched_barrier(0);
+      weigh(x);
+
+      // ---- output: the values' pairs go to LDS
+#pragma unroll
+      for (int b = 0; b < BLOCKS; ++b)
+#pragma unroll
+        for (int i = 0; i < kValueLoads; ++i) *reinterpret_cast<f32x4*>(vpairs + b * vblock + vput[i]) = vp[b][i];
+      wave_fence();
       __builtin_amdgcn_sched_barrier(0);
       constexpr int kStep = HALVES ? 1 : 2;  // fragments that lie in one group of channels whatever G is
       const float* pairs = vpairs + group * vblock + q * vpitch;
