@@ -480,6 +480,28 @@ def test_what_a_row_does_not_see_does_not_reach_it(rig, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64), ("f32", 96), ("bf16", 256)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (300, 70)])
+def test_chunks_over_many_tiles(rig, dtype, dim, window, sinks):
+    """Packed tiles, tiles of rows and those that are neither in the walk of one workgroup (enough rows to fill the
+    device) and cut into splits (few), with a page missing among the packed ones, the new rows given or written."""
+    r = rig(dtype=dtype, dim=dim, heads=4, gq=8, sequences=6, slots=6, residual=64, page=64, per_sequence=20, pages=120)
+    r.append([700, 640, 10, 0, 1000, 333])
+    holes = r.table.copy()
+    holes[0, 9] = holes[4, 12] = -1
+    gone = [np.zeros(n, bool) for n in (700, 640, 10, 0, 1000, 333)]
+    gone[0][576:640] = gone[4][768:832] = True
+    chunks = [200] * 6
+    for few in (False, True):
+        counts = [200, 0, 0, 0, 0, 0] if few else chunks
+        new = [r.tokens(m) for m in counts]
+        r.check(r.queries(sum(counts)), counts, dim ** -0.5, new=new, window=window, sinks=sinks, table=holes,
+                hidden=[np.concatenate([g, np.zeros(m, bool)]) for g, m in zip(gone, counts)])
+    r.append(chunks)
+    r.check(r.queries(400), [200, 0, 0, 0, 200, 0], dim ** -0.5, window=window, sinks=sinks)
+
+
+@pytest.mark.gpu
 def test_bounds_only_plan(rig):
     """`max_length` and the table's size change the plan, never the meaning."""
     r = rig(sequences=2, slots=2, per_sequence=20, pages=40, dim=64)
