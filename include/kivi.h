@@ -408,6 +408,7 @@ typedef struct kivi_paged_batch {
 /* Tensors of rows are [rows][heads][head_dim] of the cache's dtype: pointer, element count, and
  * elements from row to row (`*_stride`, 0: heads * head_dim). Heads lie next to each other. A stride
  * under heads * head_dim, or a count under (rows - 1) * stride + heads * head_dim, is a Shape error.
+ * The tensors of a call do not overlap.
  * Any alignment of the element type works; rows on 16 bytes are read and written faster.
  *
  * Appends the batch's new rows behind lengths[i] tokens. Up to residual_length rows a sequence may be

@@ -18,9 +18,9 @@
 // times columns of another block is ignored (keys) or zero (values). Every column keeps its own running
 // maximum and sum; they are joined at the end.
 //
-// That is for the blocks whose keys and values are all packed. The last ones (the windows, up to R and a
-// few tokens, and new rows that come with the call) go block by block: keys and values as rows of the
-// caller's type, packed tokens among them decoded, through the type's own matrix instructions.
+// That is for packed values. The last blocks (the windows, up to R and a few tokens, and new rows that come
+// with the call) go block by block, a wave each, in workgroups of their own: keys and values as rows of the
+// caller's type, packed keys among them decoded, through the type's own matrix instructions.
 #pragma once
 
 #include <algorithm>
@@ -171,7 +171,12 @@ __device__ __forceinline__ uint32_t block_at(const Walk& w, uint32_t place) {
 // One workgroup: one tile of 16 / BLOCKS rows of one (sequence, KV head), one split of its 32-token
 // blocks. In a split of packed blocks each of the four waves takes BLOCKS at a time. Per turn: the
 // keys' pairs and codes are there; the values' are fetched while the logits are computed, the next
-// turn's keys while the output is.
+// turn's keys from the softmax on.
+//
+// Measured (MI355X, 8 KV heads of 128): 64 sequences of 500 to 32768 tokens, bf16, 2 bits, 32 query heads: 536 MB in
+// 165 us and a join of 12; under a window of 4096, 32 sequences, 4 bits: 206 MB in 59 us. Two waves a SIMD
+// (216 registers) do not hide all of a turn's loads; the vector ALU is busy 45% of the time. One sequence of 1000
+// tokens: 12 us, latency.
 template <class T, int BITS, int S, int BLOCKS, bool HALVES>
 __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPlan plan, float* partial) {
   constexpr int DP = 32 * S, F = 2 * S, LW = S * BITS / 2, ROWS = 16 / BLOCKS, NT = sizeof(T) == 4 ? 3 : 2;
