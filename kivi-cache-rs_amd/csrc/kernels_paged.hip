@@ -158,7 +158,7 @@ __device__ __forceinline__ void turn_bytes(const uint32_t (&r)[4], uint32_t (&c)
 struct AppendPlan {
   uint32_t key_spans, parts;  // spans of keys, the channels of each in `parts` (1 or 4: all, or those of one q)
   uint32_t value_items, late;
-  uint32_t S_magic, octets_magic, oct_magic, words_magic, ncg_magic;  // of S, 4 S / parts, 4 S, a lane's words, D / G
+  uint32_t octets_magic, oct_magic, words_magic, ncg_magic;  // of 4 S / parts, 4 S, a lane's words, D / G
 };
 
 // Workgroup items of one (sequence, head): `parts` per key span (no two write one word), one per 32-token
@@ -563,7 +563,6 @@ hipError_t append_typed(const PagedView& c, const PagedBatch& b, const PagedRows
   p.key_spans = (uint32_t)(flushed / g.span + (g.R % g.span != 0 ? 2 : 0));
   p.parts = g.span * g.DP <= kMostStaged ? 1 : 4;
   p.value_items = (uint32_t)(((uint64_t)b.max_rows + 2 * (kPagedBlock - 1)) / kPagedBlock);
-  p.S_magic = magic_of(S);
   p.oct_magic = magic_of(4 * S);
   p.octets_magic = magic_of(4 * S / p.parts);
   p.words_magic = magic_of(BITS == 8 ? 2 * S : S * BITS / 2);

@@ -99,7 +99,6 @@ Plan plan_of(const PagedGeometry& g, const PagedBatch& b, uint32_t qh, uint64_t 
   p.chunks = rows > p.chunk.over;
   p.chunk.tile_rows = paged_chunk_rows(g);
   p.chunk.tile = paged_chunk_tokens(g);
-  p.chunk.least = 1;
   const uint64_t groups = std::max<uint64_t>(1, (uint64_t)b.rows * gq / p.chunk.tile_rows) * g.heads;  // about
   // One workgroup fills a compute unit: rounds of workgroups times the tiles of each (and two for its start and
   // end), and what a join costs, in tiles of about 3.5 us: its launch, partial sums written and read. Two sequences of 6000 rows

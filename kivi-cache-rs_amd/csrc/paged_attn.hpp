@@ -106,14 +106,12 @@ __device__ __forceinline__ Walk walk_of(const PagedAttention& a, const PagedSequ
   return w;
 }
 
-// Tiles [from, to) of split `split` of at most `splits`, each a multiple of `least` tiles, and how many
-// splits the walk takes (at least 1).
+// Tiles [from, to) of split `split` of at most `splits`, and how many splits the walk takes (at least 1).
 struct Part {
   uint32_t from, to, count;
 };
-__device__ __forceinline__ Part part_of(uint32_t tiles, uint32_t splits, uint32_t least, uint32_t split) {
-  uint32_t per = (tiles + splits - 1) / splits;
-  per = (per + least - 1) / least * least;
+__device__ __forceinline__ Part part_of(uint32_t tiles, uint32_t splits, uint32_t split) {
+  const uint32_t per = (tiles + splits - 1) / splits;
   Part p;
   p.count = tiles == 0 ? 1 : (tiles + per - 1) / per;
   p.from = split * per < tiles ? split * per : tiles;
@@ -211,7 +209,7 @@ hipError_t launch_paged_rows(const PagedAttention& a, const RowsPlan& p, float* 
 
 // Longer chunks (kernels_paged_chunk_*.hip): sequences whose KV heads have more than `over` rows.
 struct ChunkPlan {
-  uint32_t over, tile_rows, tile, splits, least;  // rows of a workgroup, tokens of a tile, splits of `least` tiles or a multiple
+  uint32_t over, tile_rows, tile, splits;  // rows of a workgroup, tokens of a tile, splits of a walk at most
 };
 // Rows of a workgroup and tokens of a tile by what the registers (512 a lane of one wave, 256 of two) and
 // LDS hold.

@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
   if (rows <= plan.over || tile_row >= rows) return;
   const uint32_t tile_end = tile_row + WAVES * 32 < rows ? tile_row + WAVES * 32 : rows;
   const Walk w = walk_of(a, s, tile_row, tile_end, gq, TT);
-  const Part part = part_of(w.tiles, splits, plan.least, split);
+  const Part part = part_of(w.tiles, splits, split);
   if (split >= part.count) return;
   // positions of the wave's first and last row and of the workgroup's first
   const int64_t at0 = w.total - s.m, first_pos = at0 + tile_row / gq;
@@ -941,10 +941,12 @@ __global__ void __launch_bounds__(paged_chunk_waves(sizeof(T), S) * 64)
   }
 }
 
-// Joins the splits of 16 rows of one KV head, a row at a time per wave, its lanes over the channels.
+// Joins the splits of 16 rows of one KV head: a wave takes four at once (one after the other they would wait
+// for memory eight times), its lanes over the channels.
 constexpr uint32_t kJoinRows = 16;
 template <class T>
 __global__ void __launch_bounds__(256) k_paged_chunk_join(PagedAttention a, ChunkPlan plan, const float* partial) {
+  constexpr int kAtOnce = kJoinRows / 4;
   const PagedGeometry& g = a.c.geo;
   const PagedSequence s = paged_sequence(a.b, g, blockIdx.z);
   const uint32_t gq = a.qh / g.heads, rows = s.m * gq, lane = threadIdx.x % 64, head = blockIdx.x % g.heads;
@@ -952,34 +954,45 @@ __global__ void __launch_bounds__(256) k_paged_chunk_join(PagedAttention a, Chun
   if (rows <= plan.over || first >= rows) return;
   const uint32_t r0 = first / plan.tile_rows * plan.tile_rows;
   const Walk w = walk_of(a, s, r0, r0 + plan.tile_rows < rows ? r0 + plan.tile_rows : rows, gq, plan.tile);
-  const uint32_t count = part_of(w.tiles, plan.splits, plan.least, 0).count;
+  const uint32_t count = part_of(w.tiles, plan.splits, 0).count;
   if (count == 1) return;
   const uint64_t all = (uint64_t)a.b.rows * a.qh;
   const float2* state = reinterpret_cast<const float2*>(partial + plan.splits * all * g.DP);
-  for (uint32_t r = first + threadIdx.x / 64; r < first + kJoinRows && r < rows; r += 4) {
-    const uint32_t token = r / gq, qhead = head * gq + r % gq;
-    const uint64_t place = (uint64_t)(s.row0 + token) * a.qh + qhead;
-    const float2 mine = lane < count ? state[lane * all + place] : make_float2(-INFINITY, 0.f);  // at most 64 splits
-    float top = mine.x;
+  const uint32_t mine = first + threadIdx.x / 64 * kAtOnce;  // this wave's first row; those past the end are the last one again
+  uint64_t place[kAtOnce];
+  float2 st[kAtOnce];
+#pragma unroll
+  for (int i = 0; i < kAtOnce; ++i) {
+    const uint32_t r = mine + i < rows ? mine + i : rows - 1;
+    place[i] = (uint64_t)(s.row0 + r / gq) * a.qh + head * gq + r % gq;
+    st[i] = lane < count ? state[lane * all + place[i]] : make_float2(-INFINITY, 0.f);  // at most 64 splits
+  }
+  float factor[kAtOnce], inv[kAtOnce];
+#pragma unroll
+  for (int i = 0; i < kAtOnce; ++i) {
+    float top = st[i].x;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    const float factor = __builtin_amdgcn_exp2f(mine.x - (top == -INFINITY ? 0.f : top));
-    float sum = factor * mine.y;
+    factor[i] = __builtin_amdgcn_exp2f(st[i].x - (top == -INFINITY ? 0.f : top));
+    float sum = factor[i] * st[i].y;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    T* out = static_cast<T*>(a.out) + (uint64_t)(s.row0 + token) * a.out_stride + (uint64_t)qhead * g.D;
-    for (uint32_t d = lane; d < (g.D + 63) / 64 * 64; d += 64) {
-      const float* p = partial + place * g.DP + (d < g.DP ? d : 0);
-      float x = 0.f;
-      for (uint32_t k = 0; k < count; k += 4) {
-        float v[4];
+    inv[i] = sum == 0.f ? 0.f : 1.f / sum;
+  }
+  for (uint32_t d = lane; d < (g.D + 63) / 64 * 64; d += 64) {
+    float x[kAtOnce] = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t k = 0; k < count; ++k) {
+      float v[kAtOnce];
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) v[i] = k + i < count ? p[(k + i) * all * g.DP] : 0.f;
+      for (int i = 0; i < kAtOnce; ++i) v[i] = partial[(k * all + place[i]) * g.DP + (d < g.DP ? d : 0)];
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) x += __shfl(factor, (int)(k + i) % 64) * v[i];
-      }
-      if (d < g.D) out[d] = (T)(x * inv);
+      for (int i = 0; i < kAtOnce; ++i) x[i] += __shfl(factor[i], (int)k) * v[i];
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const uint32_t r = mine + i;
+      if (r < rows && d < g.D)
+        static_cast<T*>(a.out)[(uint64_t)(s.row0 + r / gq) * a.out_stride + (uint64_t)(head * gq + r % gq) * g.D + d] = (T)(x[i] * inv[i]);
     }
   }
 }
