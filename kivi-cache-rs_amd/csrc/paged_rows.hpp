@@ -184,21 +184,22 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
   constexpr uint32_t kQueryPitch = DP + 4, kKeyPitch = key_pitch(S);
   extern __shared__ __align__(16) float lds[];
   const PagedGeometry& g = a.c.geo;
-  const uint32_t head = blockIdx.y, tid = threadIdx.x, lane = tid % 64;
+  const uint32_t head = blockIdx.x, sequence = blockIdx.y, tid = threadIdx.x, lane = tid % 64;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid / 64);
   const uint32_t col = lane % 16, q = lane / 16, group = col / ROWS, r = col % ROWS;
-  const PagedSequence s = paged_sequence(a.b, g, blockIdx.z);
+  const PagedSequence s = paged_sequence(a.b, g, sequence);
   const uint32_t gq = a.qh / g.heads, rows = s.m * gq;
   if (rows <= plan.over || rows > plan.most) return;
   const uint32_t places = plan.splits + plan.tails;
-  const uint32_t row0 = blockIdx.x / places * ROWS;
+  const uint32_t tiles = gridDim.z / places, row0 = blockIdx.z % tiles * ROWS;
   if (row0 >= rows) return;
   const uint32_t row1 = row0 + ROWS < rows ? row0 + ROWS : rows;
   const Walk w = walk_of(a, s, row0, row1, gq, kPagedBlock);
   const int64_t kq = paged_kq(g, s.n), vq = paged_vq(g, s.n);
   const RowsPart part = rows_part(w, vq, plan);
-  // the last blocks first: their chain of loads is the longest
-  const uint32_t turn = blockIdx.x % places;
+  // The last blocks first: their chain of loads is the longest. Then the first splits of all sequences: those that
+  // only long ones have come last, with the workgroups that find nothing to do between them.
+  const uint32_t turn = blockIdx.z / tiles;
   const bool tail = turn < plan.tails;
   if (tail ? turn >= part.tails : turn - plan.tails >= part.mains) return;
   const uint32_t split = tail ? part.mains + turn : turn - plan.tails;
@@ -684,7 +685,7 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
     }
     if (group == 0) *reinterpret_cast<f32x4*>(outs + (wave * ROWS + r) * DP + 16 * f + 4 * q) = acc[f];
   }
-  const uint64_t home = ((uint64_t)blockIdx.z * g.heads + head) * plan.stride;
+  const uint64_t home = ((uint64_t)sequence * g.heads + head) * plan.stride;
   float2* states = reinterpret_cast<float2*>(partial + (uint64_t)a.b.sequences * g.heads * plan.stride * places * DP);
   if (part.count > 1 && tid < ROWS && row0 + tid < rows) states[(home + row0 + tid) * places + split] = make_float2(all, total);
   if (tid < ROWS) inverse[tid] = total == 0.f ? 0.f : 1.f / total;  // lane r of wave 0: row r
@@ -771,7 +772,7 @@ hipError_t rows_launch(const PagedAttention& a, const RowsPlan& p, float* partia
   if (e != hipSuccess) return e;
   constexpr uint32_t kTile = 16 / BLOCKS;
   const uint32_t tiles = (p.stride + kTile - 1) / kTile;
-  hipLaunchKernelGGL(kernel, dim3(tiles * (p.splits + p.tails), g.heads, a.b.sequences), dim3(256), bytes, stream, a, p, partial);
+  hipLaunchKernelGGL(kernel, dim3(g.heads, a.b.sequences, tiles * (p.splits + p.tails)), dim3(256), bytes, stream, a, p, partial);
   hipLaunchKernelGGL(k_paged_rows_join<T>, dim3(p.stride, g.heads, a.b.sequences), dim3(256), 0, stream, a, p, partial);
   return hipGetLastError();
 }
