@@ -64,7 +64,7 @@ Plan plan_of(const PagedGeometry& g, const PagedBatch& b, uint32_t qh, uint64_t 
     const uint32_t most[2] = {decode, kRowsMost};
     uint32_t over = 0;
     // Where most sequences have to be near the longest chunk, one launch takes all rows of any number (an empty
-    // launch and its join cost 7 us: 16 sequences of five drafted tokens 104 -> 95 us).
+    // launch and its join cost 7 us: 16 sequences of five drafted tokens 104 -> 94 us).
     const bool alike = (uint64_t)b.rows * 2 > (uint64_t)b.sequences * b.max_rows;
     for (uint32_t i = 0; i < 2 && over < rows && over < kRowsMost; ++i) {
       if (alike && rows > kRowsMost) break;
@@ -79,7 +79,7 @@ Plan plan_of(const PagedGeometry& g, const PagedBatch& b, uint32_t qh, uint64_t 
       const auto cut = [&](uint64_t n, uint64_t cap) {
         const uint64_t blocks = std::max<uint64_t>(1, (n + kPagedBlock - 1) / kPagedBlock);
         // one to eight turns a wave (what surrounds the turns costs about one), more where there are many: 64
-        // sequences to 32768 tokens 178 us with at most eight, 187 with four
+        // sequences to 32768 tokens 171 us with at most eight, 178 with four, 182 with sixteen
         const uint64_t turns = std::clamp<uint64_t>(blocks * heads * tiles / turn / 1024, 1, 8);
         const uint64_t least = std::max({turns * turn, blocks * heads * tiles / kRowsWorkgroups, (blocks + cap - 1) / cap});
         r.least = (uint32_t)((least + turn - 1) / turn * turn);

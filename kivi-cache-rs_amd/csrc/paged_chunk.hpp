@@ -54,8 +54,8 @@ struct Mma<float> {
 // Rows are what they are and need one.
 //
 // Bound by the vector ALU (softmax and decoding, 380 instructions per wave and plain tile) beside the matrix
-// cores (48 instructions): 2048 rows over 16384 cached tokens, bf16, 2 bits, 32 query heads of 128: 900 to
-// 945 us, 620 to 650 TFLOP/s (one loop for all kinds of tiles: 1370 us, half its instructions addresses and spilled scalars).
+// cores (48 instructions): 2048 rows over 16384 cached tokens, bf16, 2 bits, 32 query heads of 128: 890 to
+// 945 us, 620 to 655 TFLOP/s (one loop for all kinds of tiles: 1370 us, half its instructions addresses and spilled scalars).
 // Halves of a tile at different times in a SIMD's two waves: 1030 us, against 980 then.
 template <class T>
 constexpr int kKeyTerms = sizeof(T) == 2 ? 2 : 1;

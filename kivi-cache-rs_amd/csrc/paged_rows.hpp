@@ -174,9 +174,8 @@ __device__ __forceinline__ uint32_t block_at(const Walk& w, uint32_t place) {
 // turn's keys from the softmax on.
 //
 // Measured (MI355X, 8 KV heads of 128): 64 sequences of 500 to 32768 tokens, bf16, 2 bits, 32 query heads: 536 MB in
-// 165 us and a join of 12; under a window of 4096, 32 sequences, 4 bits: 206 MB in 59 us. Two waves a SIMD
-// (216 registers) do not hide all of a turn's loads; the vector ALU is busy 45% of the time. One sequence of 1000
-// tokens: 12 us, latency.
+// 171 us (3.1 TB/s) and a join of 12; under a window of 4096, 32 sequences, 4 bits: 206 MB in 56 us. The vector ALU is
+// busy 43% of the time, 1.3 waves a SIMD on average (216 registers: two fit). One sequence of 1000 tokens: 12 us, latency.
 template <class T, int BITS, int S, int BLOCKS, bool HALVES>
 __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPlan plan, float* partial) {
   constexpr int DP = 32 * S, F = 2 * S, LW = S * BITS / 2, ROWS = 16 / BLOCKS, NT = sizeof(T) == 4 ? 3 : 2;
@@ -198,7 +197,8 @@ __global__ void __launch_bounds__(256, 2) k_paged_rows(PagedAttention a, RowsPla
   const int64_t kq = paged_kq(g, s.n), vq = paged_vq(g, s.n);
   const RowsPart part = rows_part(w, vq, plan);
   // The last blocks first: their chain of loads is the longest. Then the first splits of all sequences: those that
-  // only long ones have come last, with the workgroups that find nothing to do between them.
+  // only long ones have come last, with the workgroups that find nothing to do between them (windowed decode of 32
+  // sequences 59 -> 56 us, splits fastest against this).
   const uint32_t turn = blockIdx.z / tiles;
   const bool tail = turn < plan.tails;
   if (tail ? turn >= part.tails : turn - plan.tails >= part.mains) return;
