@@ -64,7 +64,7 @@ Plan plan_of(const PagedGeometry& g, const PagedBatch& b, uint32_t qh, uint64_t 
     const uint32_t most[2] = {decode, kRowsMost};
     uint32_t over = 0;
     // Where most sequences have to be near the longest chunk, one launch takes all rows of any number (an empty
-    // launch and its join cost 7 us: 16 sequences of five drafted tokens 104 -> 94 us).
+    // launch and its join cost 7 us).
     const bool alike = (uint64_t)b.rows * 2 > (uint64_t)b.sequences * b.max_rows;
     for (uint32_t i = 0; i < 2 && over < rows && over < kRowsMost; ++i) {
       if (alike && rows > kRowsMost) break;
@@ -102,7 +102,7 @@ Plan plan_of(const PagedGeometry& g, const PagedBatch& b, uint32_t qh, uint64_t 
   const uint64_t groups = std::max<uint64_t>(1, (uint64_t)b.rows * gq / p.chunk.tile_rows) * g.heads;  // about
   // One workgroup fills a compute unit: rounds of workgroups times the tiles of each (and two for its start and
   // end), and what a join costs, in tiles of about 3.5 us: its launch, partial sums written and read. Two sequences of 6000 rows
-  // (375 groups) over 18 tiles: 1 split 126 us, 2 splits 181.
+  // (375 groups) over 18 tiles: 1 split 117 us, 2 splits 124 and a join of 33.
   const auto chunk_splits = [&](uint64_t n) {
     const uint64_t tiles = std::max<uint64_t>(1, (n + p.chunk.tile - 1) / p.chunk.tile);
     uint64_t best = 1, least_cost = ~(uint64_t)0;
